@@ -1,0 +1,61 @@
+// The number types of the vocabulary operators (embedding lookup and
+// gradient, distillation, sampling): 32-bit floats and the two 16-bit formats,
+// all computed with in 32 bits or more and rounded once when they are stored.
+#pragma once
+#include "base.hxx"
+
+#ifdef __CUDACC__
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+BEGIN_MGPU_NAMESPACE
+namespace detail {
+
+template<typename real_t>
+struct is_model_real : std::false_type { };
+template<> struct is_model_real<float> : std::true_type { };
+template<> struct is_model_real<__half> : std::true_type { };
+template<> struct is_model_real<__nv_bfloat16> : std::true_type { };
+
+MGPU_DEVICE __forceinline__ float to_f32(float x) { return x; }
+MGPU_DEVICE __forceinline__ float to_f32(__half x) { return __half2float(x); }
+MGPU_DEVICE __forceinline__ float to_f32(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+
+// One rounding to nearest, ties to even.
+template<typename real_t>
+MGPU_DEVICE __forceinline__ real_t from_f32(float x);
+template<>
+MGPU_DEVICE __forceinline__ float from_f32<float>(float x) { return x; }
+template<>
+MGPU_DEVICE __forceinline__ __half from_f32<__half>(float x) {
+  return __float2half_rn(x);
+}
+template<>
+MGPU_DEVICE __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// `count` neighbouring values that are loaded and stored as one word of up to
+// 16 bytes (two words for a pack of 32).
+template<typename real_t, int count>
+struct MGPU_ALIGN((sizeof(real_t) * count > 16 ? 16 : sizeof(real_t) * count))
+pack_t {
+  real_t v[count];
+};
+
+// The widest pack, in elements of `size` bytes, that divides `width` and that
+// every row starts on a boundary of: rows `stride` elements apart from `base`.
+inline int pack_limit(const void* base, int64_t stride, int64_t width,
+  int size) {
+  int pack = 16 / size;
+  while(pack > 1 && ((uintptr_t)base % (size_t)(pack * size) ||
+    stride % pack || width % pack)) pack /= 2;
+  return pack;
+}
+
+} // namespace detail
+END_MGPU_NAMESPACE
+
+#endif // __CUDACC__

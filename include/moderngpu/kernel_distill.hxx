@@ -1,0 +1,3 @@
+// The implementation lives under b200/.
+#pragma once
+#include "b200/distill.hxx"

@@ -41,6 +41,9 @@ enum {
 /* Element types. */
 enum { MGPU_B200_F32 = 0, MGPU_B200_F64 = 1, MGPU_B200_I32 = 2, MGPU_B200_I64 = 3 };
 
+/* 16-bit element types, of the vocabulary operators only. */
+enum { MGPU_B200_F16 = 4, MGPU_B200_BF16 = 5 };
+
 /* Reduction operators: mgpu::plus_t, maximum_t, minimum_t
  * (reference: src/moderngpu/operators.hxx:94-124). */
 enum { MGPU_B200_PLUS = 0, MGPU_B200_MAX = 1, MGPU_B200_MIN = 2 };
@@ -257,6 +260,90 @@ size_t mgpu_b200_scan_workspace_bytes(int dtype, int count);
 int mgpu_b200_scan(int dtype, int inclusive, const void* input_device,
   int count, void* output_device, void* total_device, void* workspace_device,
   size_t workspace_bytes, void* stream);
+
+/*
+ * Vocabulary operators (no counterpart in the reference): what a language
+ * model does with its tokens at either end, on the primitives above. `dtype`
+ * is MGPU_B200_F32, _F16 or _BF16, `token_dtype` MGPU_B200_I32 or _I64.
+ * Matrices are row by row with `stride` elements from row to row, dense where
+ * no stride is given. Sums are held in 32 bits (sampling: 64) and rounded once.
+ * Arrays have to be aligned to their elements; rows that start on 16-byte
+ * boundaries are fastest.
+ *
+ * mgpu_b200_embedding_lookup (interval_gather with rows for items):
+ *   output[i] = scale * table[tokens[i]], a row of `width` elements;
+ * a token outside of [0, rows) gives a row of zeros. The output must not
+ * overlap the table. count + rows < 2^31 - 65536, width <= 2^20.
+ *
+ * mgpu_b200_embedding_gradient (segreduce with rows for items, the positions
+ * sorted by token): output[r] = scale * sum of grad[i] over the positions i
+ * with tokens[i] == r, summed in the order of the positions (the same call
+ * gives the same bits). Tokens outside of [0, rows) are left out. With
+ * accumulate == 0 every row of the output is written, those without a token
+ * with zeros; otherwise the sums are added to the output and other rows are
+ * not touched. output_dtype is dtype or MGPU_B200_F32. Workspace:
+ * mgpu_b200_embedding_gradient_workspace_bytes(...), 128-byte aligned, one
+ * for each call in flight; 0 for sizes out of range.
+ */
+int mgpu_b200_embedding_lookup(int dtype, const void* table_device, int rows,
+  int width, int64_t stride, int token_dtype, const void* tokens_device,
+  int count, float scale, void* output_device, void* stream);
+
+size_t mgpu_b200_embedding_gradient_workspace_bytes(int count, int rows,
+  int width, int accumulate);
+
+int mgpu_b200_embedding_gradient(int dtype, const void* grad_device,
+  int64_t stride, int width, int token_dtype, const void* tokens_device,
+  int count, int rows, float scale, int accumulate, int output_dtype,
+  void* output_device, void* workspace_device, size_t workspace_bytes,
+  void* stream);
+
+/*
+ * Distillation from a teacher's top logits. Row i has the student's logits s
+ * over the vocabulary and `entries` (at most 1024) pairs of a token j_k and the
+ * teacher's logit t_k for it (tokens and teacher: count x entries, dense;
+ * teacher_dtype as dtype). With p = softmax of t_k / T over the row's entries
+ * and q = softmax of s / T over the vocabulary,
+ *   losses[i] = T^2 * sum_k p_k (log p_k - log q[j_k])
+ *   grad[i][v] = weights[i] * T * (q_v - sum of the p_k with j_k == v).
+ * An entry whose token is outside of [0, vocabulary) is unused; a token may
+ * occur in several entries. A row without an entry above -infinity, a row
+ * whose logits are all -infinity and a row of weight 0 have loss 0 and
+ * gradient 0 (the logits of the first and the last are not read). `weights`
+ * may be NULL: 1 for every row. grad may be logits itself (same stride), and
+ * must not overlap it otherwise. T > 0.
+ */
+int mgpu_b200_distill_loss(int dtype, const void* logits_device, int64_t stride,
+  int count, int vocabulary, int token_dtype, const void* tokens_device,
+  int teacher_dtype, const void* teacher_device, int entries, float temperature,
+  float* losses_device, void* stream);
+
+int mgpu_b200_distill_loss_gradient(int dtype, const void* logits_device,
+  int64_t stride, int count, int vocabulary, int token_dtype,
+  const void* tokens_device, int teacher_dtype, const void* teacher_device,
+  int entries, float temperature, const float* weights_device,
+  float* losses_device, void* grad_device, int64_t grad_stride, void* stream);
+
+/*
+ * One token for each row of logits, drawn by the given numbers u in [0, 1)
+ * (a scan of the row's weights and a search in it, behind a selection). With
+ * the weights w_v = exp((x_v - max x) / T):
+ *   1. the top_k greatest logits are kept (top_k <= 0: all);
+ *   2. of these, greatest first, the shortest run whose weight is at least
+ *      top_p times the weight of them all (top_p >= 1: all; at least one);
+ *   3. of these, those with w_v >= min_p (the greatest always is);
+ *   4. of these, in the order of the vocabulary, the first token whose running
+ *      weight exceeds u times the weight of all that are left.
+ * Equal logits are ordered by index. T == 0 takes the greatest logit. A row
+ * with a NaN or without a logit above -infinity gives -1. Each setting is one
+ * number for all rows, or an array with one for each where its pointer is not
+ * NULL; numbers out of range in an array act as the nearest one in range.
+ */
+int mgpu_b200_sample_tokens(int dtype, const void* logits_device,
+  int64_t stride, int count, int vocabulary, const float* uniforms_device,
+  float temperature, const float* temperatures_device, int top_k,
+  const int* top_ks_device, float top_p, const float* top_ps_device,
+  float min_p, const float* min_ps_device, int* tokens_device, void* stream);
 
 /*
  * Multi-GPU layer (no counterpart in the reference, which is single-device).

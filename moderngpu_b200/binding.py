@@ -84,6 +84,8 @@ def load_library():
     lib.mgpu_b200_debug_set_wait_limit_ns.restype = ctypes.c_uint64
     lib.mgpu_b200_debug_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     _declare_optional(lib)
+    from . import vocabulary
+    vocabulary.declare(lib)
     _lib = lib
     return lib
 

@@ -19,6 +19,7 @@ NVCC_FLAGS = [
     "--expt-extended-lambda", "--expt-relaxed-constexpr",
     "-O3", "-lineinfo",
     "-Xcompiler", "-fPIC", "-shared",
+    "--threads", "0",
 ]
 
 
