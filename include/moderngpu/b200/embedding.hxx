@@ -5,12 +5,12 @@
 //
 // The lookup is interval_gather with whole rows for elements. The gradient is
 // a segmented reduction with whole rows for items: the positions are sorted by
-// token (stable, so that equal tokens keep the order of their positions), each
-// row of the table is a segment of the sorted positions, and a row that no
-// token names is an empty segment. The work of both is cut as segreduce cuts
-// it, by merge path over the sorted positions and the ends of the rows, so a
-// token that fills half of the batch and a hundred thousand rows without a
-// token cost every CTA the same.
+// token (stable, so that equal tokens keep the order of their positions), and
+// the sorted positions are cut into tiles of equal length, whatever the lengths
+// of the runs of equal tokens. A run that crosses tiles leaves a partial sum in
+// each; the CTA that comes last adds them up, in order. Rows that no token
+// names are segments without items: a kernel of their own zeroes them while the
+// sort, which needs few SMs, is running.
 //
 // A token outside of [0, rows) stands for no row (padding): the lookup gives
 // zeros for it, the gradient leaves its position out.
@@ -21,6 +21,9 @@
 #include "runtime.hxx"
 #include "real_types.hxx"
 #include "scan.hxx"
+#ifdef __CUDACC__
+#include <cooperative_groups.h>
+#endif
 
 BEGIN_MGPU_NAMESPACE
 
@@ -88,16 +91,18 @@ void embedding_lookup_enqueue(const real_t* table, int64_t rows, int width,
 ////////////////////////////////////////////////////////////////////////////////
 // Positions sorted by token: a stable radix sort, least significant digit
 // first, of the pairs (row, position). Tokens that name no row become the key
-// `rows` and end up behind all others.
+// `rows` and end up behind all others. Two forms: one cluster of CTAs that keeps
+// the pairs in shared memory (up to 131,072 positions, one launch), and three
+// launches a digit for any number.
 
 enum { token_sort_nt = 256, token_sort_vt = 16,
   token_sort_nv = token_sort_nt * token_sort_vt, token_digit_bits = 9,
   token_digits = 1 << token_digit_bits };
 
-inline int token_sort_passes(int rows) {
-  int bits = 0;
+inline int token_bits(int rows) {
+  int bits = 1;
   while(bits < 32 && ((uint64_t)rows >> bits)) ++bits;   // keys 0 .. rows
-  return bits ? div_up(bits, (int)token_digit_bits) : 1;
+  return bits;
 }
 
 // The keys of the first pass come from the caller's tokens.
@@ -192,48 +197,200 @@ token_scatter_k(source_t source, int count, int shift, int tiles,
   }
 }
 
-////////////////////////////////////////////////////////////////////////////////
-// Gradient.
+// Each warp owns a run of neighbouring pairs, 32 at a time in order, and has
+// them in registers between the passes. Lanes with equal digits find one another
+// by a match vote; a pair's place is the number of pairs with a smaller digit,
+// of the CTAs and warps before it with the same digit, and of its equals before
+// it in its own warp.
+enum { token_cluster_nt = 1024, token_cluster_most = 8 };
 
-// Where a tile starts: `entry` sorted positions and `row` rows are before it.
-struct MGPU_ALIGN(8) embedding_cut_t { int entry, row; };
+template<int vt>
+struct token_cluster_shared_t {
+  enum { warps = token_cluster_nt / 32, nv = token_cluster_nt * vt };
+  uint32_t keys[nv];
+  int positions[nv];
+  uint16_t seen[warps][token_digits];
+  int totals[token_digits];
+  int starts[token_digits];
+  int warp_sums[token_digits / 32];
+};
 
-enum { embedding_tile = 64 };
+template<int vt, typename token_t>
+__global__ void __launch_bounds__(token_cluster_nt)
+token_cluster_sort_k(token_keys_t<token_t> source, int count, int bits,
+  int passes, int ctas, uint32_t* keys_out, int* positions_out, int* counters,
+  int64_t num_counters) {
+  enum { nt = token_cluster_nt, warps = nt / 32 };
+  extern __shared__ __align__(16) char token_cluster_memory[];
+  typedef token_cluster_shared_t<vt> shared_t;
+  shared_t& shared = *(shared_t*)token_cluster_memory;
+  auto cluster = cooperative_groups::this_cluster();
+  // The kernel that follows zeroes the rows without a token meanwhile.
+  ptx::grid_launch_dependents();
 
-// Tile t holds the elements [64 t, 64 t + 64) of the merge of the sorted keys
-// with the ends of the rows 0, 1, ..., rows - 1 (the end of a row comes after
-// its entries). keys[e] + e rises strictly, so the entries in front of the
-// merged place d are those with keys[e] + e < d: one binary search for a tile.
-// With `accumulate` rows without entries have nothing to write, and tiles are
-// 64 entries each.
-template<int nt>
-__global__ void __launch_bounds__(nt)
-embedding_cuts_k(const uint32_t* keys, int count, int rows, int accumulate,
-  int tiles, embedding_cut_t* cuts) {
-  int t = (int)(blockIdx.x * nt + threadIdx.x);
-  if(t > tiles) return;
-  int64_t place = (int64_t)t * embedding_tile;
-  int lo = 0, hi = count;
-  if(accumulate) {
-    // Entries with a row of the table.
-    while(lo < hi) {
-      int mid = (int)(((int64_t)lo + hi) / 2);
-      if(keys[mid] < (uint32_t)rows) lo = mid + 1; else hi = mid;
+  int rank = (int)cluster.block_rank(), tid = (int)threadIdx.x;
+  int warp = tid / 32, lane = tid % 32;
+  int rounds = div_up(div_up(count, ctas * warps), 32);
+  int per_warp = rounds * 32, per_cta = per_warp * warps;
+  int first = rank * per_cta + warp * per_warp;
+  for(int64_t i = rank * nt + tid; i < num_counters; i += ctas * nt)
+    counters[i] = 0;
+
+  uint32_t keys[vt];
+  int positions[vt];
+  #pragma unroll
+  for(int j = 0; j < vt; ++j) {
+    int i = first + j * 32 + lane;
+    bool live = j < rounds && i < count;
+    keys[j] = live ? source.key(i) : 0;
+    positions[j] = i;
+  }
+  int digit_bits = div_up(bits, passes), digits = 1 << digit_bits;
+  for(int pass = 0; pass < passes; ++pass) {
+    int shift = pass * digit_bits;
+    for(int d = tid; d < warps * token_digits / 2; d += nt)
+      ((uint32_t*)shared.seen)[d] = 0;
+    __syncthreads();
+    int places[vt];
+    #pragma unroll
+    for(int j = 0; j < vt; ++j) {
+      if(j < rounds) {
+        bool live = first + j * 32 + lane < count;
+        int digit = live ? (int)((keys[j] >> shift) & (digits - 1)) : digits;
+        unsigned peers = __match_any_sync(0xffffffffu, digit);
+        int ahead = __popc(peers & ((1u << lane) - 1));
+        int before = live ? shared.seen[warp][digit] : 0;
+        __syncwarp();
+        if(live && !ahead)
+          shared.seen[warp][digit] = (uint16_t)(before + __popc(peers));
+        __syncwarp();
+        places[j] = before + ahead;
+      }
     }
-    int entry = place < lo ? (int)place : lo;
-    cuts[t] = embedding_cut_t { entry, entry < lo ? (int)keys[entry] : rows };
-  } else {
-    while(lo < hi) {
-      int mid = (int)(((int64_t)lo + hi) / 2);
-      if((int64_t)keys[mid] + mid < place && keys[mid] < (uint32_t)rows)
-        lo = mid + 1;
-      else
-        hi = mid;
+    __syncthreads();
+    // A thread for each digit: the warps' counts become places in the CTA.
+    if(tid < digits) {
+      int sum = 0;
+      #pragma unroll 8
+      for(int w = 0; w < warps; ++w) {
+        int c = shared.seen[w][tid];
+        shared.seen[w][tid] = (uint16_t)sum;
+        sum += c;
+      }
+      shared.totals[tid] = sum;
     }
-    int64_t row = place - lo;
-    cuts[t] = embedding_cut_t { lo, row < rows ? (int)row : rows };
+    cluster.sync();
+    int before = 0, all = 0, upto = 0;
+    if(tid < token_digits) {
+      if(tid < digits)
+        for(int r = 0; r < ctas; ++r) {
+          int c = cluster.map_shared_rank(&shared, r)->totals[tid];
+          if(r < rank) before += c;
+          all += c;
+        }
+      upto = all;
+      #pragma unroll
+      for(int offset = 1; offset < 32; offset *= 2) {
+        int y = __shfl_up_sync(0xffffffffu, upto, offset);
+        if(lane >= offset) upto += y;
+      }
+      if(31 == lane) shared.warp_sums[warp] = upto;
+    }
+    __syncthreads();
+    if(tid < digits) {
+      for(int w = 0; w < warp; ++w) upto += shared.warp_sums[w];
+      shared.starts[tid] = upto - all + before;
+    }
+    __syncthreads();
+    bool done = pass + 1 == passes;
+    #pragma unroll
+    for(int j = 0; j < vt; ++j) {
+      if(j < rounds && first + j * 32 + lane < count) {
+        int digit = (int)((keys[j] >> shift) & (digits - 1));
+        int to = shared.starts[digit] + shared.seen[warp][digit] + places[j];
+        if(done) {
+          keys_out[to] = keys[j];
+          positions_out[to] = positions[j];
+        } else {
+          int r = to / per_cta;
+          shared_t* there = cluster.map_shared_rank(&shared, r);
+          there->keys[to - r * per_cta] = keys[j];
+          there->positions[to - r * per_cta] = positions[j];
+        }
+      }
+    }
+    // Also: no CTA leaves, or counts again, while another reads its totals.
+    cluster.sync();
+    if(!done) {
+      #pragma unroll
+      for(int j = 0; j < vt; ++j) {
+        int i = warp * per_warp + j * 32 + lane;
+        if(j < rounds && rank * per_cta + i < count) {
+          keys[j] = shared.keys[i];
+          positions[j] = shared.positions[i];
+        }
+      }
+    }
   }
 }
+
+template<int nt>
+__global__ void __launch_bounds__(nt) embedding_clear_k(int* counters,
+  int64_t n) {
+  for(int64_t i = (int64_t)blockIdx.x * nt + threadIdx.x; i < n;
+    i += (int64_t)gridDim.x * nt) counters[i] = 0;
+}
+
+////////////////////////////////////////////////////////////////////////////////
+// Rows without a token. CTA b owns the rows b, b + gridDim.x, ... (tokens crowd
+// at low numbers), marks those among them that the tokens name in a bitmap, and
+// zeroes the others.
+
+enum { embedding_zero_nt = 512, embedding_zero_rows = 32768 };
+
+template<int pack, typename out_t, typename token_t>
+__global__ void __launch_bounds__(embedding_zero_nt)
+embedding_zero_k(token_keys_t<token_t> source, int count, int width, int lanes,
+  out_t* output) {
+  enum { nt = embedding_zero_nt };
+  typedef pack_t<out_t, pack> word_t;
+  __shared__ uint32_t named[embedding_zero_rows / 32];
+  word_t zero;
+  #pragma unroll
+  for(int j = 0; j < pack; ++j) zero.v[j] = from_f32<out_t>(0.0f);
+  uint32_t ctas = gridDim.x, cta = blockIdx.x;
+  int owned = (int)(((uint32_t)source.rows + ctas - 1 - cta) / ctas);
+  int lane = (int)threadIdx.x & (lanes - 1), group = (int)threadIdx.x / lanes;
+  for(int base = 0; base < owned; base += embedding_zero_rows) {
+    int here = min(owned - base, (int)embedding_zero_rows);
+    for(int i = threadIdx.x; i < div_up(here, 32); i += nt) named[i] = 0;
+    __syncthreads();
+    #pragma unroll 4
+    for(int64_t i = threadIdx.x; i < count; i += nt) {
+      uint32_t row = source.key((int)i);
+      uint32_t place = row / ctas;
+      if(row - place * ctas == cta && row < (uint32_t)source.rows) {
+        int at = (int)place - base;
+        if(at >= 0 && at < here) atomicOr(&named[at / 32], 1u << (at % 32));
+      }
+    }
+    __syncthreads();
+    for(int i = group; i < here; i += nt / lanes) {
+      if(named[i / 32] >> (i % 32) & 1) continue;
+      out_t* to = output + ((size_t)(base + i) * ctas + cta) * width;
+      for(int c = lane * pack; c < width; c += lanes * pack)
+        *(word_t*)(to + c) = zero;
+    }
+    __syncthreads();
+  }
+  // Where this kernel runs beside the sort: the sums that follow need both.
+  ptx::grid_dependency_wait();
+}
+
+////////////////////////////////////////////////////////////////////////////////
+// Sums.
+
+enum { embedding_most_tile = 256 };
 
 template<typename out_t, int pack>
 MGPU_DEVICE __forceinline__ void store_row_part(out_t* to,
@@ -254,205 +411,346 @@ MGPU_DEVICE __forceinline__ void store_row_part(out_t* to,
   }
 }
 
-// One CTA per tile and slab of nt * pack columns; every thread walks the
-// tile's entries for its own columns with the running sum in registers. A row
-// that began in an earlier tile, and one that goes on in a later tile, leaves
-// its sum in `head` and `tail` for embedding_join_k.
+// A partial sum, as words of up to 16 bytes.
+template<int pack>
+struct part_t {
+  enum { piece = pack > 4 ? 4 : pack };
+  pack_t<float, piece> words[pack / piece];
+};
+
+// One CTA per tile and slab of nt * pack columns; every thread walks the tile's
+// entries for its own columns, `batch` rows in flight, with the running sum in
+// registers. Bound by HBM: each row of grad is read once.
+//
+// parts holds two sums for each tile: of the run that was begun in an earlier
+// tile (2 t), and of one that begins here and goes on (2 t + 1). counters, one
+// for each tile and slab, start at 0 and count the sums of the run that begins
+// in the tile.
 template<int nt, int pack, typename real_t, typename out_t>
 __global__ void __launch_bounds__(nt)
 embedding_sum_k(const real_t* grad, int64_t stride, int width,
-  const uint32_t* keys, const int* positions, const embedding_cut_t* cuts,
-  float scale, int accumulate, out_t* output, float* head, float* tail) {
+  const uint32_t* keys, const int* positions, int count, int rows, int tile_size,
+  float scale, int accumulate, out_t* output, float* parts, int* counters) {
   typedef pack_t<real_t, pack> word_t;
-  __shared__ uint32_t tile_keys[embedding_tile];
-  __shared__ int tile_positions[embedding_tile];
-  __shared__ int carried;
-  int tile = (int)blockIdx.x;
-  embedding_cut_t from = cuts[tile], to = cuts[tile + 1];
-  int entries = to.entry - from.entry;
-  for(int e = threadIdx.x; e < entries; e += nt) {
-    tile_keys[e] = keys[from.entry + e];
-    tile_positions[e] = positions[from.entry + e];
+  enum { batch = 8 };
+  __shared__ uint32_t tile_keys[embedding_most_tile];
+  __shared__ int tile_positions[embedding_most_tile];
+  __shared__ int told;
+  ptx::grid_dependency_wait();
+  int tile = (int)blockIdx.x, tid = (int)threadIdx.x;
+  int begin = tile * tile_size, end = min(begin + tile_size, count);
+  int entries = end - begin;
+  for(int e = tid; e < entries; e += nt) {
+    tile_keys[e] = keys[begin + e];
+    tile_positions[e] = positions[begin + e];
   }
-  if(!threadIdx.x)
-    carried = from.entry > 0 && from.row < to.row &&
-      keys[from.entry - 1] == (uint32_t)from.row;
+  uint32_t row = keys[begin];
+  if(row >= (uint32_t)rows) return;
+  bool carried = begin > 0 && keys[begin - 1] == row;
+  uint32_t next = end < count ? keys[end] : (uint32_t)rows;
   __syncthreads();
-  int column = (int)(blockIdx.y * nt + threadIdx.x) * pack;
-  if(column >= width) return;
+  // Entries that name no row are the last ones of all.
+  while(tile_keys[entries - 1] >= (uint32_t)rows) --entries;
+  bool goes_on = tile_keys[entries - 1] == next;
 
-  float sum[pack], zero[pack];
+  int column = (int)(blockIdx.y * nt + tid) * pack;
+  bool live = column < width;
+  float sum[pack];
   #pragma unroll
-  for(int j = 0; j < pack; ++j) sum[j] = zero[j] = 0;
-  int row = from.row;
-  bool first = carried, some = false;
-  auto finish = [&]() {
-    if(first) {
-      #pragma unroll
-      for(int j = 0; j < pack; ++j)
-        head[(size_t)tile * width + column + j] = sum[j];
-    } else if(some || !accumulate)
-      store_row_part<out_t, pack>(output + (size_t)row * width + column, sum,
-        scale, 0 != accumulate);
-    first = some = false;
-    #pragma unroll
-    for(int j = 0; j < pack; ++j) sum[j] = 0;
-  };
-  auto skip_to = [&](int next) {
-    if(!accumulate)
-      for(int r = row + 1; r < next; ++r)
-        store_row_part<out_t, pack>(output + (size_t)r * width + column, zero,
-          scale, false);
-    row = next;
-  };
-  for(int e = 0; e < entries; ++e) {
-    int key = (int)tile_keys[e];
-    if(key != row) {
-      finish();
-      skip_to(key);
-    }
-    word_t word = *(const word_t*)(grad + (int64_t)tile_positions[e] * stride +
-      column);
-    some = true;
-    #pragma unroll
-    for(int j = 0; j < pack; ++j) sum[j] += to_f32(word.v[j]);
-  }
-  if(row < to.row) {
-    finish();
-    skip_to(to.row);
-  } else if(some) {
+  for(int j = 0; j < pack; ++j) sum[j] = 0;
+  auto keep_part = [&](int slot) {
+    if(!live) return;
+    part_t<pack> part;
     #pragma unroll
     for(int j = 0; j < pack; ++j)
-      tail[(size_t)tile * width + column + j] = sum[j];
+      part.words[j / part_t<pack>::piece].v[j % part_t<pack>::piece] = sum[j];
+    *(part_t<pack>*)(parts + (size_t)slot * width + column) = part;
+  };
+  bool head = carried;
+  for(int e = 0; e < entries; e += batch) {
+    word_t words[batch];
+    #pragma unroll
+    for(int i = 0; i < batch; ++i)
+      if(e + i < entries && live)
+        words[i] = *(const word_t*)(grad +
+          (int64_t)tile_positions[e + i] * stride + column);
+    #pragma unroll
+    for(int i = 0; i < batch; ++i) {
+      if(e + i < entries) {
+        uint32_t key = tile_keys[e + i];
+        if(key != row) {
+          if(head)
+            keep_part(2 * tile);
+          else if(live)
+            store_row_part<out_t, pack>(output + (size_t)row * width + column,
+              sum, scale, 0 != accumulate);
+          head = false;
+          row = key;
+          #pragma unroll
+          for(int j = 0; j < pack; ++j) sum[j] = 0;
+        }
+        #pragma unroll
+        for(int j = 0; j < pack; ++j) sum[j] += to_f32(words[i].v[j]);
+      }
+    }
+  }
+  if(head || goes_on)
+    keep_part(2 * tile + (head ? 0 : 1));
+  else if(live)
+    store_row_part<out_t, pack>(output + (size_t)row * width + column, sum,
+      scale, 0 != accumulate);
+
+  // The runs that cross tiles: the one begun earlier, and the one that goes on
+  // (they are the same one where it fills the tile: `head` is still set).
+  for(int which = 0; which < 2; ++which) {
+    if(which ? !(goes_on && !head) : !carried) continue;
+    uint32_t key = which ? row : tile_keys[0];
+    // Its first and last tile: threads look at the tiles' borders.
+    int from = tile, to = tile;
+    if(!which) {
+      bool found = false;
+      for(int b = tile; !found; b -= nt) {
+        int border = b - tid;
+        bool out = border <= 0 || keys[(size_t)border * tile_size - 1] != key;
+        if(!tid) told = -1;
+        __syncthreads();
+        if(out) atomicMax(&told, max(border, 0));
+        __syncthreads();
+        found = told >= 0;
+        from = told;
+        __syncthreads();
+      }
+    }
+    if(which || head) {
+      if(goes_on) {
+        bool found = false;
+        for(int b = tile + 1; !found; b += nt) {
+          int64_t border = (int64_t)b + tid;
+          bool out = border * tile_size >= count ||
+            keys[border * tile_size] != key;
+          if(!tid) told = 0x7fffffff;
+          __syncthreads();
+          if(out) atomicMin(&told, (int)border - 1);
+          __syncthreads();
+          found = told != 0x7fffffff;
+          to = told;
+          __syncthreads();
+        }
+      }
+    }
+    // This CTA's sum is stored; the last to say so adds up.
+    __syncthreads();
+    if(!tid) {
+      __threadfence();
+      told = atomicAdd(counters + (size_t)from * gridDim.y + blockIdx.y, 1);
+      __threadfence();
+    }
+    __syncthreads();
+    bool last = told == to - from;
+    __syncthreads();
+    if(!last || !live) continue;
+    float total[pack];
+    #pragma unroll
+    for(int j = 0; j < pack; ++j) total[j] = 0;
+    for(int t = from; t <= to; t += batch) {
+      part_t<pack> some[batch];
+      #pragma unroll
+      for(int i = 0; i < batch; ++i)
+        if(t + i <= to) {
+          const part_t<pack>* at = (const part_t<pack>*)(parts +
+            (size_t)(2 * (t + i) + (t + i == from)) * width + column);
+          some[i] = *at;
+        }
+      #pragma unroll
+      for(int i = 0; i < batch; ++i)
+        if(t + i <= to) {
+          #pragma unroll
+          for(int j = 0; j < pack; ++j)
+            total[j] += some[i].words[j / part_t<pack>::piece].v[
+              j % part_t<pack>::piece];
+        }
+    }
+    store_row_part<out_t, pack>(output + (size_t)key * width + column, total,
+      scale, 0 != accumulate);
   }
 }
 
-// The first row that ends in a tile, where it began in an earlier one: the
-// sums of the tiles before it, in order, and its own.
-template<int nt, typename out_t>
-__global__ void __launch_bounds__(nt)
-embedding_join_k(int width, const uint32_t* keys, const embedding_cut_t* cuts,
-  float scale, int accumulate, out_t* output, const float* head,
-  const float* tail) {
-  int tile = (int)blockIdx.x;
-  embedding_cut_t from = cuts[tile], to = cuts[tile + 1];
-  if(!(from.entry > 0 && from.row < to.row &&
-    keys[from.entry - 1] == (uint32_t)from.row)) return;
-  // The earliest tile that holds an entry of the row: tiles between it and
-  // this one hold nothing else.
-  int lo = 0, hi = from.entry;
-  while(lo < hi) {
-    int mid = (int)(((int64_t)lo + hi) / 2);
-    if(keys[mid] < (uint32_t)from.row) lo = mid + 1; else hi = mid;
-  }
-  int begin = tile - 1;
-  int a = 0, b = tile;              // last cut with entry <= lo
-  while(a < b) {
-    int mid = (int)(((int64_t)a + b) / 2);
-    if(cuts[mid + 1].entry <= lo) a = mid + 1; else b = mid;
-  }
-  begin = a;
-  for(int c = blockIdx.y * nt + threadIdx.x; c < width; c += gridDim.y * nt) {
-    float sum = 0;
-    for(int t = begin; t < tile; ++t) sum += tail[(size_t)t * width + c];
-    sum += head[(size_t)tile * width + c];
-    float part[1] = { sum };
-    store_row_part<out_t, 1>(output + (size_t)from.row * width + c, part, scale,
-      0 != accumulate);
-  }
-}
-
-// Scratch: the pairs of two passes, the digit counts with the scan's own
-// scratch, the tiles' cuts and the sums of rows that cross tiles.
+// Sizes and scratch of a call: the sorted pairs (two sets and the digit counts
+// with their scan where one cluster does not take them), the partial sums and
+// their counters.
 struct embedding_plan_t {
-  int tiles, sort_tiles, passes;
-  size_t keys[2], positions[2], counts, scan, cuts, head, tail, bytes;
+  int tile_size, tiles, slab_limit, vt, ctas, sort_tiles;
+  size_t keys[2], positions[2], counts, scan, parts, counters, bytes;
 
-  embedding_plan_t(int count, int rows, int width, bool accumulate) {
-    int64_t merged = accumulate ? (int64_t)count : (int64_t)count + rows;
-    tiles = (int)div_up(merged, (int64_t)embedding_tile);
-    sort_tiles = (int)div_up((int64_t)count, (int64_t)token_sort_nv);
-    passes = token_sort_passes(rows);
+  embedding_plan_t(int count, int rows, int width) {
+    // About eight tiles for each SM; fewer entries than 8 in a tile would make
+    // partial sums a third of the traffic.
+    tile_size = 8;
+    while(tile_size < embedding_most_tile &&
+      (int64_t)tile_size * 1184 < count) tile_size *= 2;
+    tiles = div_up(count, tile_size);
+    slab_limit = div_up(width, 32);        // a slab has 32 columns at least
+    vt = count <= 4 * token_cluster_nt * token_cluster_most ? 4 : 16;
+    ctas = 0;
+    if(count <= vt * token_cluster_nt * token_cluster_most) {
+      ctas = 1;
+      while(ctas < token_cluster_most && ctas * 2048 < count) ctas *= 2;
+    }
+    sort_tiles = ctas ? 0 : div_up(count, (int)token_sort_nv);
     size_t at = 0;
     auto take = [&](size_t n) {
       size_t here = at;
       at += (n + 127) / 128 * 128;
       return here;
     };
-    for(int i = 0; i < 2; ++i) {
+    for(int i = 0; i < (ctas ? 1 : 2); ++i) {
       keys[i] = take(4 * (size_t)count);
       positions[i] = take(4 * (size_t)count);
     }
+    if(ctas) {
+      keys[1] = keys[0];
+      positions[1] = positions[0];
+    }
     int cells = sort_tiles * token_digits;
     counts = take(4 * (size_t)cells);
-    scan = take(scan_workspace_bytes<typename scan_default_tuning<int>::type,
-      int>(cells));
-    cuts = take(sizeof(embedding_cut_t) * ((size_t)tiles + 1));
-    head = take(4 * (size_t)tiles * width);
-    tail = take(4 * (size_t)tiles * width);
+    scan = take(ctas ? 0 : scan_workspace_bytes<
+      typename scan_default_tuning<int>::type, int>(cells));
+    parts = take(8 * (size_t)tiles * width);
+    counters = take(4 * (size_t)tiles * slab_limit);
     bytes = at;
   }
 };
+
+// Launch that may begin while its predecessor in the stream still runs.
+template<typename... params_t, typename... args_t>
+void launch_beside(void (*kernel)(params_t...), dim3 grid, int nt,
+  cudaStream_t stream, args_t... args) {
+  cudaLaunchConfig_t config = { };
+  config.gridDim = grid;
+  config.blockDim = dim3((unsigned)nt);
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  throw_on_error(cudaLaunchKernelEx(&config, kernel, params_t(args)...));
+}
+
+template<int vt, typename token_t>
+void token_cluster_sort(const embedding_plan_t& plan,
+  token_keys_t<token_t> source, int count, uint32_t* keys, int* positions,
+  int* counters, int64_t num_counters, cudaStream_t stream) {
+  auto kernel = token_cluster_sort_k<vt, token_t>;
+  const int smem = (int)sizeof(token_cluster_shared_t<vt>);
+  set_dynamic_smem<token_cluster_shared_t<vt>, token_t>(kernel, smem);
+  cudaLaunchConfig_t config = { };
+  config.gridDim = dim3((unsigned)plan.ctas);
+  config.blockDim = dim3(token_cluster_nt);
+  config.dynamicSmemBytes = (size_t)smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)plan.ctas;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  int bits = token_bits(source.rows);
+  throw_on_error(cudaLaunchKernelEx(&config, kernel, source, count, bits,
+    div_up(bits, (int)token_digit_bits), plan.ctas, keys, positions, counters,
+    num_counters));
+}
+
+// The widest pack for `width` columns on both sides, as a constant for f.
+template<typename func_t>
+void with_pack(int pack, func_t f) {
+  switch(pack) {
+    case 8: f(std::integral_constant<int, 8>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    default: f(std::integral_constant<int, 1>()); break;
+  }
+}
 
 template<typename real_t, typename out_t, typename token_t>
 void embedding_gradient_enqueue(const real_t* grad, int64_t stride, int width,
   const token_t* tokens, int count, int rows, float scale, bool accumulate,
   out_t* output, void* workspace, cudaStream_t stream) {
   if(!rows || !width || (accumulate && !count)) return;
-  embedding_plan_t plan(count, rows, width, accumulate);
+  embedding_plan_t plan(count, rows, width);
   char* base = (char*)workspace;
   uint32_t* keys[2] = { (uint32_t*)(base + plan.keys[0]),
     (uint32_t*)(base + plan.keys[1]) };
   int* positions[2] = { (int*)(base + plan.positions[0]),
     (int*)(base + plan.positions[1]) };
-  int* counts = (int*)(base + plan.counts);
-  embedding_cut_t* cuts = (embedding_cut_t*)(base + plan.cuts);
-  float* head = (float*)(base + plan.head);
-  float* tail = (float*)(base + plan.tail);
+  float* parts = (float*)(base + plan.parts);
+  int* counters = (int*)(base + plan.counters);
+  int64_t num_counters = (int64_t)plan.tiles * plan.slab_limit;
+  token_keys_t<token_t> source { tokens, rows };
 
   int into = 0;
-  if(count) {
+  if(count && plan.ctas) {
+    if(4 == plan.vt)
+      token_cluster_sort<4>(plan, source, count, keys[0], positions[0],
+        counters, num_counters, stream);
+    else
+      token_cluster_sort<16>(plan, source, count, keys[0], positions[0],
+        counters, num_counters, stream);
+  } else if(count) {
     typedef scan_route_t<empty_t, int, int*, int*> route_t;
-    auto pass = [&](auto source, int shift, int to) {
-      token_count_k<<<plan.sort_tiles, token_sort_nt, 0, stream>>>(source,
+    int* counts = (int*)(base + plan.counts);
+    auto pass = [&](auto from, int shift, int to) {
+      token_count_k<<<plan.sort_tiles, token_sort_nt, 0, stream>>>(from,
         count, shift, plan.sort_tiles, counts);
       scan_dispatch<route_t, scan_type_exc, int>(counts,
         plan.sort_tiles * token_digits, counts, plus_t<int>(),
         discard_iterator_t<int>(), base + plan.scan, stream);
-      token_scatter_k<<<plan.sort_tiles, token_sort_nt, 0, stream>>>(source,
+      token_scatter_k<<<plan.sort_tiles, token_sort_nt, 0, stream>>>(from,
         count, shift, plan.sort_tiles, counts, keys[to], positions[to]);
     };
-    pass(token_keys_t<token_t> { tokens, rows }, 0, 0);
-    for(int p = 1; p < plan.passes; ++p, into ^= 1)
+    embedding_clear_k<256><<<148, 256, 0, stream>>>(counters, num_counters);
+    int passes = div_up(token_bits(rows), (int)token_digit_bits);
+    pass(source, 0, 0);
+    for(int p = 1; p < passes; ++p, into ^= 1)
       pass(sorted_keys_t { keys[into], positions[into] },
         p * token_digit_bits, into ^ 1);
+    throw_on_error(cudaGetLastError());
   }
-  embedding_cuts_k<256><<<div_up(plan.tiles + 1, 256), 256, 0, stream>>>(
-    keys[into], count, rows, accumulate, plan.tiles, cuts);
-  // A pack of 8 columns is stored as two words where the sums are 32 bits wide.
   int out_pack = pack_limit(output, width, width, (int)sizeof(out_t));
+  if(!accumulate)
+    with_pack(out_pack, [&](auto tag) {
+      enum { vt = sizeof(out_t) == 2 || (int)decltype(tag)::value < 8 ?
+        (int)decltype(tag)::value : 4 };
+      int lanes = 1;
+      while(lanes < embedding_zero_nt && lanes * vt < width) lanes *= 2;
+      // Beside the sort, which was launched behind everything before it; without
+      // one this kernel may begin no earlier than any other.
+      dim3 grid((unsigned)min(rows, 296));
+      if(count)
+        launch_beside(embedding_zero_k<vt, out_t, token_t>, grid,
+          embedding_zero_nt, stream, source, count, width, lanes, output);
+      else
+        embedding_zero_k<vt, out_t, token_t><<<grid, embedding_zero_nt, 0,
+          stream>>>(source, count, width, lanes, output);
+    });
+  if(!count) return;
+  // A pack of 8 columns is stored as two words where the sums are 32 bits wide.
   if(16 / (int)sizeof(out_t) == out_pack) out_pack = 8;
-  int pack = min(pack_limit(grad, stride, width, (int)sizeof(real_t)),
-    out_pack);
-  auto launch = [&](auto tag) {
-    enum { nt = 128 };
-    enum { vt = decltype(tag)::value };
-    dim3 grid((unsigned)plan.tiles, (unsigned)div_up(width, nt * vt));
-    embedding_sum_k<nt, vt, real_t, out_t><<<grid, nt, 0, stream>>>(grad,
-      stride, width, keys[into], positions[into], cuts, scale, accumulate,
-      output, head, tail);
-  };
-  switch(pack) {
-    case 8: launch(std::integral_constant<int,
-      (sizeof(real_t) == 2 ? 8 : 4)>()); break;
-    case 4: launch(std::integral_constant<int, 4>()); break;
-    case 2: launch(std::integral_constant<int, 2>()); break;
-    default: launch(std::integral_constant<int, 1>()); break;
-  }
-  embedding_join_k<256, out_t><<<dim3((unsigned)plan.tiles,
-    (unsigned)min(div_up(width, 256), 64)), 256, 0, stream>>>(width, keys[into],
-    cuts, scale, accumulate, output, head, tail);
-  throw_on_error(cudaGetLastError());
+  with_pack(min(pack_limit(grad, stride, width, (int)sizeof(real_t)), out_pack),
+    [&](auto tag) {
+      enum { vt = sizeof(real_t) == 2 || (int)decltype(tag)::value < 8 ?
+        (int)decltype(tag)::value : 4 };
+      auto launch = [&](auto threads) {
+        enum { nt = decltype(threads)::value };
+        launch_beside(embedding_sum_k<nt, vt, real_t, out_t>,
+          dim3((unsigned)plan.tiles, (unsigned)div_up(width, nt * vt)), nt,
+          stream, grad, stride, width, keys[into], positions[into], count, rows,
+          plan.tile_size, scale, (int)accumulate, output, parts, counters);
+      };
+      if(width <= 32 * vt) launch(std::integral_constant<int, 32>());
+      else if(width <= 128 * vt) launch(std::integral_constant<int, 128>());
+      else launch(std::integral_constant<int, 256>());
+    });
 }
 
 } // namespace detail
@@ -483,8 +781,8 @@ void embedding_gradient(const real_t* grad, int64_t stride, int width,
     detail::is_model_real<out_t>::value,
     "embedding_gradient takes float, __half or __nv_bfloat16");
   detail::throw_on_device_status();
-  mem_t<char> workspace(detail::embedding_plan_t(count, rows, width,
-    accumulate).bytes, context);
+  mem_t<char> workspace(detail::embedding_plan_t(count, rows, width).bytes,
+    context);
   detail::embedding_gradient_enqueue(grad, stride, width, tokens, count, rows,
     scale, accumulate, output, workspace.data(), context.stream());
 }

@@ -2,7 +2,8 @@
 // gradient, distillation, sampling): 32-bit floats and the two 16-bit formats,
 // all computed with in 32 bits or more and rounded once when they are stored.
 #pragma once
-#include "base.hxx"
+#include "runtime.hxx"
+#include <atomic>
 
 #ifdef __CUDACC__
 #include <cuda_bf16.h>
@@ -53,6 +54,19 @@ inline int pack_limit(const void* base, int64_t stride, int64_t width,
   while(pack > 1 && ((uintptr_t)base % (size_t)(pack * size) ||
     stride % pack || width % pack)) pack /= 2;
   return pack;
+}
+
+// Allows a kernel its dynamic shared memory, once per device. tag_t...: what
+// tells its instantiations apart.
+template<typename... tag_t, typename kernel_t>
+void set_dynamic_smem(kernel_t kernel, int bytes) {
+  static std::atomic<bool> done[64] = { };
+  int device = 0;
+  throw_on_error(cudaGetDevice(&device));
+  if(device < 64 && done[device].load(std::memory_order_acquire)) return;
+  throw_on_error(cudaFuncSetAttribute(kernel,
+    cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if(device < 64) done[device].store(true, std::memory_order_release);
 }
 
 } // namespace detail

@@ -160,8 +160,7 @@ int mgpu_b200_embedding_lookup(int dtype, const void* table_device, int rows,
 size_t mgpu_b200_embedding_gradient_workspace_bytes(int count, int rows,
   int width, int accumulate) {
   if(bad_embedding_sizes(count, rows, width)) return 0;
-  size_t bytes = detail::embedding_plan_t(count, rows, width,
-    0 != accumulate).bytes;
+  size_t bytes = detail::embedding_plan_t(count, rows, width).bytes;
   return bytes ? bytes : 128;
 }
 

@@ -17,6 +17,7 @@ from .binding import (_DTYPES, _check, _on, _require_cuda, _stream, _workspace,
 F16, BF16 = 4, 5
 _REALS = {torch.float32: _DTYPES[torch.float32], torch.float16: F16,
           torch.bfloat16: BF16}
+_MOST = 0x7fffffff
 _TOKENS = {torch.int32: _DTYPES[torch.int32],
            torch.int64: _DTYPES[torch.int64]}
 
@@ -52,6 +53,18 @@ def declare(lib):
         c_void_p]
 
 
+# The address of the current stream without the Stream object around it, which
+# costs as much as the launch of a small kernel; the public way where a torch
+# does not have it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(device):
+    if _raw_stream is None or device.index is None:
+        return _stream(device)
+    return _raw_stream(device.index)
+
+
 def _require(t, name, dtypes, device=None):
     """A dense CUDA tensor of one of the dtypes, on the call's device."""
     _require_cuda(t, name)
@@ -63,7 +76,7 @@ def _require(t, name, dtypes, device=None):
 
 
 def _matrix(t, name, dtypes, device=None):
-    """Checks a matrix whose rows are dense; returns its row stride."""
+    """Checks a matrix whose rows are dense; returns (rows, width, stride)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA tensor" % name)
     if t.dtype not in dtypes:
@@ -73,20 +86,23 @@ def _matrix(t, name, dtypes, device=None):
         raise ValueError("%s must be on %s" % (name, device))
     if t.dim() != 2:
         raise ValueError("%s must have two dimensions" % name)
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    (rows, width), (stride, step) = t.shape, t.stride()
+    if width > 1 and step != 1:
         raise ValueError("the rows of %s must be contiguous" % name)
-    if t.shape[0] < 2:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
+    if rows < 2:
+        stride = width
+    if stride < width:
         raise ValueError("the rows of %s must not overlap" % name)
-    return t.stride(0)
+    if rows > _MOST or width > _MOST:
+        raise ValueError("%s is too large: %d x %d" % (name, rows, width))
+    return rows, width, stride
 
 
-def _fits(**sizes):
+def _fits(n, name):
     """The library's sizes are 32 bits wide; ctypes would cut off the rest."""
-    for name, n in sizes.items():
-        if n > 0x7fffffff:
-            raise ValueError("%s is too large: %d" % (name, n))
+    if n > _MOST:
+        raise ValueError("%s is too large: %d" % (name, n))
+    return n
 
 
 def _shaped(out, name, shape, dtypes, device):
@@ -117,16 +133,16 @@ def embedding_lookup(table, tokens, scale=1.0, out=None):
     of any shape; out: tokens.shape + (width,), of the table's dtype.
     """
     lib = load_library()
-    stride = _matrix(table, "table", _REALS)
-    _require(tokens, "tokens", _TOKENS, table.device)
-    _fits(rows=table.shape[0], width=table.shape[1], tokens=tokens.numel())
-    out = _shaped(out, "out", tuple(tokens.shape) + (table.shape[1],),
-                  (table.dtype,), table.device)
-    with _on(table.device):
+    dtype, device = table.dtype, table.device
+    rows, width, stride = _matrix(table, "table", _REALS)
+    _require(tokens, "tokens", _TOKENS, device)
+    count = _fits(tokens.numel(), "tokens")
+    out = _shaped(out, "out", tokens.shape + (width,), (dtype,), device)
+    with _on(device):
         _check(lib.mgpu_b200_embedding_lookup(
-            _REALS[table.dtype], table.data_ptr(), table.shape[0],
-            table.shape[1], stride, _TOKENS[tokens.dtype], tokens.data_ptr(),
-            tokens.numel(), scale, out.data_ptr(), _stream(table.device)))
+            _REALS[dtype], table.data_ptr(), rows, width, stride,
+            _TOKENS[tokens.dtype], tokens.data_ptr(), count, scale,
+            out.data_ptr(), _stream_of(device)))
     return out
 
 
@@ -146,38 +162,38 @@ def embedding_gradient(grad, tokens, rows, scale=1.0, out=None,
     _require(tokens, "tokens", _TOKENS, grad.device)
     if grad.dim() < 1 or tuple(grad.shape[:-1]) != tuple(tokens.shape):
         raise ValueError("grad must have one row for each token")
-    width, count = grad.shape[-1], tokens.numel()
+    device = grad.device
+    width, count = grad.shape[-1], _fits(tokens.numel(), "tokens")
+    _fits(rows, "rows")
     if grad.dim() != 2:
         if not grad.is_contiguous():
             raise ValueError("grad must be contiguous, or a matrix")
         grad = grad.view(count, width)
-    stride = _matrix(grad, "grad", _REALS)
-    _fits(rows=rows, width=width, tokens=count)
+    _, _, stride = _matrix(grad, "grad", _REALS)
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     out = _shaped(out, "out", (rows, width), (grad.dtype, torch.float32),
-                  grad.device)
+                  device)
     if workspace is None:
         # A size out of range asks for 0 bytes here and is refused below.
         workspace = _call_workspace(
-            grad.device, lib.mgpu_b200_embedding_gradient_workspace_bytes(
+            device, lib.mgpu_b200_embedding_gradient_workspace_bytes(
                 count, rows, width, int(accumulate)))
     else:
-        _require(workspace, "workspace", (torch.uint8,), grad.device)
-    with _on(grad.device):
+        _require(workspace, "workspace", (torch.uint8,), device)
+    with _on(device):
         _check(lib.mgpu_b200_embedding_gradient(
             _REALS[grad.dtype], grad.data_ptr(), stride, width,
             _TOKENS[tokens.dtype], tokens.data_ptr(), count, rows, scale,
             int(accumulate), _REALS[out.dtype], out.data_ptr(),
-            workspace.data_ptr(), workspace.numel(), _stream(grad.device)))
+            workspace.data_ptr(), workspace.numel(), _stream_of(device)))
     return out
 
 
-def _teacher(logits, teacher_tokens, teacher_logits):
-    _fits(rows=logits.shape[0], vocabulary=logits.shape[1])
-    _require(teacher_tokens, "teacher_tokens", _TOKENS, logits.device)
-    _require(teacher_logits, "teacher_logits", _REALS, logits.device)
-    if teacher_tokens.dim() != 2 or teacher_tokens.shape[0] != logits.shape[0]:
+def _teacher(count, device, teacher_tokens, teacher_logits):
+    _require(teacher_tokens, "teacher_tokens", _TOKENS, device)
+    _require(teacher_logits, "teacher_logits", _REALS, device)
+    if teacher_tokens.dim() != 2 or teacher_tokens.shape[0] != count:
         raise ValueError("teacher_tokens must have one row for each of logits")
     if teacher_logits.shape != teacher_tokens.shape:
         raise ValueError("teacher_logits must have teacher_tokens' shape")
@@ -195,16 +211,16 @@ def distill_loss(logits, teacher_tokens, teacher_logits, temperature=1.0,
     teacher_logits: of the same shape, any of the three dtypes.
     """
     lib = load_library()
-    stride = _matrix(logits, "logits", _REALS)
-    entries = _teacher(logits, teacher_tokens, teacher_logits)
-    count, vocabulary = logits.shape
-    out = _shaped(out, "out", (count,), (torch.float32,), logits.device)
-    with _on(logits.device):
+    device = logits.device
+    count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    entries = _teacher(count, device, teacher_tokens, teacher_logits)
+    out = _shaped(out, "out", (count,), (torch.float32,), device)
+    with _on(device):
         _check(lib.mgpu_b200_distill_loss(
             _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
             _TOKENS[teacher_tokens.dtype], teacher_tokens.data_ptr(),
             _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
-            temperature, out.data_ptr(), _stream(logits.device)))
+            temperature, out.data_ptr(), _stream_of(device)))
     return out
 
 
@@ -219,10 +235,9 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
     `logits` itself, which then holds the gradient.
     """
     lib = load_library()
-    stride = _matrix(logits, "logits", _REALS)
-    entries = _teacher(logits, teacher_tokens, teacher_logits)
-    count, vocabulary = logits.shape
     device = logits.device
+    count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    entries = _teacher(count, device, teacher_tokens, teacher_logits)
     loss = _shaped(loss, "loss", (count,), (torch.float32,), device)
     if row_weights is not None:
         _require(row_weights, "row_weights", (torch.float32,), device)
@@ -231,7 +246,7 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
     if out is None:
         out = torch.empty((count, vocabulary), dtype=logits.dtype,
                           device=device)
-    out_stride = _matrix(out, "out", (logits.dtype,), device)
+    _, _, out_stride = _matrix(out, "out", (logits.dtype,), device)
     if out.shape != logits.shape:
         raise ValueError("out must have the logits' shape")
     with _on(device):
@@ -241,16 +256,16 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
             _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
             temperature, None if row_weights is None else
             row_weights.data_ptr(), loss.data_ptr(), out.data_ptr(),
-            out_stride, _stream(device)))
+            out_stride, _stream_of(device)))
     return loss, out
 
 
-def _setting(value, name, dtype, logits):
+def _setting(value, name, dtype, count, device):
     """(number, address) of a setting: one of the two counts."""
     if not isinstance(value, torch.Tensor):
         return value, None
-    _require(value, name, (dtype,), logits.device)
-    if tuple(value.shape) != (logits.shape[0],):
+    _require(value, name, (dtype,), device)
+    if tuple(value.shape) != (count,):
         raise ValueError("%s must have one number for each row" % name)
     return 0, value.data_ptr()
 
@@ -268,20 +283,20 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
     without a logit above -infinity gives -1.
     """
     lib = load_library()
-    stride = _matrix(logits, "logits", _REALS)
-    count, vocabulary = logits.shape
-    _fits(rows=count, vocabulary=vocabulary)
-    _require(uniform, "uniform", (torch.float32,), logits.device)
+    device = logits.device
+    count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    _require(uniform, "uniform", (torch.float32,), device)
     if tuple(uniform.shape) != (count,):
         raise ValueError("uniform must have one number for each row")
-    t, t_rows = _setting(temperature, "temperature", torch.float32, logits)
-    k, k_rows = _setting(top_k, "top_k", torch.int32, logits)
-    p, p_rows = _setting(top_p, "top_p", torch.float32, logits)
-    m, m_rows = _setting(min_p, "min_p", torch.float32, logits)
-    out = _shaped(out, "out", (count,), (torch.int32,), logits.device)
-    with _on(logits.device):
+    t, t_rows = _setting(temperature, "temperature", torch.float32, count,
+                         device)
+    k, k_rows = _setting(top_k, "top_k", torch.int32, count, device)
+    p, p_rows = _setting(top_p, "top_p", torch.float32, count, device)
+    m, m_rows = _setting(min_p, "min_p", torch.float32, count, device)
+    out = _shaped(out, "out", (count,), (torch.int32,), device)
+    with _on(device):
         _check(lib.mgpu_b200_sample_tokens(
             _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
             uniform.data_ptr(), t, t_rows, k, k_rows, p, p_rows, m, m_rows,
-            out.data_ptr(), _stream(logits.device)))
+            out.data_ptr(), _stream_of(device)))
     return out
