@@ -117,6 +117,27 @@ __device__ __forceinline__ void bulk_wait() {
   asm volatile("cp.async.bulk.wait_group %0;" :: "n"(pending) : "memory");
 }
 
+// Copy of 4, 8 or 16 bytes global -> shared memory by the issuing thread, which
+// groups its copies and waits for all but the `pending` newest groups. Only the
+// issuing thread may read the data without a further barrier.
+template<int bytes>
+__device__ __forceinline__ void cp_async(void* smem_dst, const void* gmem_src) {
+  static_assert(4 == bytes || 8 == bytes || 16 == bytes, "4, 8 or 16 bytes");
+  if constexpr (16 == bytes)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+      :: "r"(smem_addr(smem_dst)), "l"(gmem_src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
+      :: "r"(smem_addr(smem_dst)), "l"(gmem_src), "n"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template<int pending>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" :: "n"(pending) : "memory");
+}
+
 // Programmatic dependent launch: a kernel launched with the programmatic
 // stream-serialization attribute may start while its predecessor in the
 // stream is still running; it must call grid_dependency_wait() before it

@@ -46,6 +46,31 @@ pack_t {
   real_t v[count];
 };
 
+// A store of data that this kernel does not read again: first to leave the L2.
+template<typename real_t, int count>
+MGPU_DEVICE __forceinline__ void store_streaming(pack_t<real_t, count>* to,
+  const pack_t<real_t, count>& word) {
+  enum { size = sizeof(pack_t<real_t, count>) };
+  static_assert(2 == size || 4 == size || 8 == size || 16 == size, "one word");
+  if constexpr (16 == size) {
+    uint4 bits;
+    memcpy(&bits, &word, 16);
+    __stcs((uint4*)to, bits);
+  } else if constexpr (8 == size) {
+    uint2 bits;
+    memcpy(&bits, &word, 8);
+    __stcs((uint2*)to, bits);
+  } else if constexpr (4 == size) {
+    uint32_t bits;
+    memcpy(&bits, &word, 4);
+    __stcs((uint32_t*)to, bits);
+  } else {
+    uint16_t bits;
+    memcpy(&bits, &word, 2);
+    __stcs((unsigned short*)to, bits);
+  }
+}
+
 // The widest pack, in elements of `size` bytes, that divides `width` and that
 // every row starts on a boundary of: rows `stride` elements apart from `base`.
 inline int pack_limit(const void* base, int64_t stride, int64_t width,
@@ -54,6 +79,17 @@ inline int pack_limit(const void* base, int64_t stride, int64_t width,
   while(pack > 1 && ((uintptr_t)base % (size_t)(pack * size) ||
     stride % pack || width % pack)) pack /= 2;
   return pack;
+}
+
+// A pack of 1, 2, 4 or 8 elements as a constant for f.
+template<typename func_t>
+void with_pack(int pack, func_t f) {
+  switch(pack) {
+    case 8: f(std::integral_constant<int, 8>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    default: f(std::integral_constant<int, 1>()); break;
+  }
 }
 
 // Allows a kernel its dynamic shared memory, once per device. tag_t...: what

@@ -29,6 +29,7 @@ def sources():
 
 def _inputs():
     deps = sources()
+    deps += glob.glob(os.path.join(PKG_DIR, "csrc", "*.h"))
     deps += glob.glob(os.path.join(ROOT, "include", "*.h"))
     deps += glob.glob(os.path.join(ROOT, "include", "moderngpu", "*.hxx"))
     deps += glob.glob(os.path.join(ROOT, "include", "moderngpu", "b200", "*.hxx"))
