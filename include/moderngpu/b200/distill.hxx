@@ -10,15 +10,20 @@
 //
 // An entry whose token lies outside of the vocabulary is unused. A row without
 // a used entry (or with none above -infinity), a row whose logits are all
-// -infinity, and a row of weight 0 have loss 0 and gradient 0; the logits of
-// the first and the last are not read.
+// -infinity, and a row of weight 0 have loss 0 and gradient 0, whatever else
+// they hold.
 #pragma once
 #include "runtime.hxx"
 #include "real_types.hxx"
+#include "ptx.hxx"
+#include "tile_state.hxx"
+#ifdef __CUDACC__
+#include <cooperative_groups.h>
+#endif
 
 BEGIN_MGPU_NAMESPACE
 
-enum { distill_max_entries = 1024 };
+enum { distill_max_entries = 1024, distill_max_cluster = 8 };
 
 #ifdef __CUDACC__
 
@@ -46,132 +51,676 @@ MGPU_DEVICE __forceinline__ peak_sum_t merge(peak_sum_t a, peak_sum_t b,
     b.sum * exp2_fast((b.peak - base) * c) };
 }
 
-template<int nt>
-MGPU_DEVICE __forceinline__ peak_sum_t cta_merge(peak_sum_t x, float c,
-  peak_sum_t* shared) {
+MGPU_DEVICE __forceinline__ peak_sum_t warp_merge(peak_sum_t x, float c) {
   #pragma unroll
   for(int offset = 16; offset; offset /= 2) {
     peak_sum_t y { __shfl_xor_sync(0xffffffffu, x.peak, offset),
       __shfl_xor_sync(0xffffffffu, x.sum, offset) };
     x = merge(x, y, c);
   }
-  if(0 == threadIdx.x % 32) shared[threadIdx.x / 32] = x;
-  __syncthreads();
-  x = shared[0];
-  for(int w = 1; w < nt / 32; ++w) x = merge(x, shared[w], c);
-  __syncthreads();
   return x;
 }
 
-template<int nt>
-MGPU_DEVICE __forceinline__ float cta_sum(float x, float* shared) {
-  #pragma unroll
-  for(int offset = 16; offset; offset /= 2)
-    x += __shfl_xor_sync(0xffffffffu, x, offset);
-  if(0 == threadIdx.x % 32) shared[threadIdx.x / 32] = x;
-  __syncthreads();
-  x = shared[0];
-  for(int w = 1; w < nt / 32; ++w) x += shared[w];
-  __syncthreads();
-  return x;
-}
+// The teacher's arrays, of any type: read once per row, by few threads.
+struct distill_teacher_t {
+  const void* tokens;
+  const void* logits;
+  int wide, kind;                  // 64-bit tokens; 0 float, 1 half, 2 bfloat16
+  int entries;
+  MGPU_DEVICE int64_t token(int64_t i) const {
+    return wide ? ((const int64_t*)tokens)[i] : ((const int*)tokens)[i];
+  }
+  MGPU_DEVICE float logit(int64_t i) const {
+    switch(kind) {
+      case 1: return to_f32(((const __half*)logits)[i]);
+      case 2: return to_f32(((const __nv_bfloat16*)logits)[i]);
+    }
+    return ((const float*)logits)[i];
+  }
+};
+inline int teacher_kind(const float*) { return 0; }
+inline int teacher_kind(const __half*) { return 1; }
+inline int teacher_kind(const __nv_bfloat16*) { return 2; }
 
-// One CTA per row: the teacher's entries, one pass over the logits for the
-// maximum and the sum, the loss, and with want_grad a second pass for the
-// gradient.
-template<int nt, int pack, bool want_grad, typename real_t, typename teacher_t,
-  typename token_t>
-__global__ void __launch_bounds__(nt)
-distill_k(const real_t* logits, int64_t stride, int vocabulary,
-  const token_t* tokens, const teacher_t* teacher, int entries,
-  float temperature, const float* weights, float* losses, real_t* grad,
-  int64_t grad_stride) {
+// A cluster of CTAs per row, each with a part of it. The first `held` words of
+// 16 bytes of each thread are requested at once and stay in registers, so that a
+// row which fits (32 KB a CTA) is read once and its gradient written from there;
+// what goes beyond is read again, from the L2. Bound by HBM bytes: one read, and
+// with want_grad one write, of the logits. The only exchange is one of a peak
+// and a sum for each warp.
+template<int nt, int pack, bool want_grad, typename real_t>
+__global__ void __launch_bounds__(nt, 768 / nt)
+distill_k(const real_t* logits, int64_t stride, int vocabulary, int ctas,
+  distill_teacher_t teacher, float temperature, const float* weights,
+  float* losses, real_t* grad, int64_t grad_stride) {
   typedef pack_t<real_t, pack> word_t;
-  __shared__ float p[distill_max_entries];
-  __shared__ float student[distill_max_entries];
-  __shared__ int at[distill_max_entries];
-  __shared__ peak_sum_t merged[nt / 32];
-  __shared__ float summed[nt / 32];
+  enum { warps = nt / 32, held = 8, parts = distill_max_cluster * warps };
+  extern __shared__ int distill_memory[];
+  __shared__ peak_sum_t part[parts];
+  __shared__ peak_sum_t teacher_part[warps];
+  __shared__ float loss_part[warps];
+  auto cluster = cooperative_groups::this_cluster();
+  if(ctas > 1) ptx::cluster_arrive_relaxed();
 
-  int64_t row = blockIdx.x;
-  int tid = threadIdx.x;
+  int entries = teacher.entries;
+  int* at = distill_memory;                  // -1: unused
+  float* p = (float*)(distill_memory + entries);
+  float* student = p + entries;
+  int tid = (int)threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int rank = (int)blockIdx.x % ctas;
+  int64_t row = (int64_t)blockIdx.x / ctas;
   const real_t* x = logits + row * stride;
+  real_t* g = grad + row * grad_stride;
   const float c = 1.4426950408889634f / temperature;
-  float weight = weights ? weights[row] : 1.0f;
 
-  // The teacher's distribution. A NaN stays one.
+  // Whole words between the row's first and last 16-byte border, an equal part
+  // of them for each CTA; the elements outside, one to a thread of the first.
+  int head = min((int)((16 - (uintptr_t)x % 16) % 16 / sizeof(real_t)) % pack,
+    vocabulary);
+  int words = (vocabulary - head) / pack;
+  int tail = vocabulary - head - words * pack;
+  const word_t* x_words = (const word_t*)(x + head);
+  int per_cta = div_up(words, ctas);
+  int begin = min(rank * per_cta, words), end = min(begin + per_cta, words);
+  int edge = rank ? -1 : tid < head ? tid :
+    tid < head + tail ? vocabulary - tail + (tid - head) : -1;
+
+  word_t word[held];
+  #pragma unroll
+  for(int i = 0; i < held; ++i) {
+    int w = begin + i * nt + tid;
+    if(w < end) word[i] = x_words[w];
+    else {
+      #pragma unroll
+      for(int j = 0; j < pack; ++j) word[i].v[j] = from_f32<real_t>(-INFINITY);
+    }
+  }
+  float edge_value = edge >= 0 ? to_f32(x[edge]) : -INFINITY;
+
+  // The teacher's distribution, meanwhile, and the student's logits at its
+  // tokens: all of them in the first CTA, for the loss, and a CTA's own, for the
+  // gradient. They are read before the barrier below, the gradient is written
+  // behind it: it may take the logits' place. A NaN stays one.
+  auto own = [&](int j) {
+    if(j < head || j >= vocabulary - tail) return 0 == rank;
+    int w = (j - head) / pack;
+    return w >= begin && w < end;
+  };
+  float weight = weights ? weights[row] : 1.0f;
   peak_sum_t t { -INFINITY, 0.0f };
   for(int k = tid; k < entries; k += nt) {
-    int64_t j = (int64_t)tokens[row * entries + k];
+    int64_t j = teacher.token(row * entries + k);
     bool used = j >= 0 && j < vocabulary && weight != 0;
+    float logit = used ? teacher.logit(row * entries + k) : -INFINITY;
     at[k] = used ? (int)j : -1;
-    p[k] = used ? to_f32(teacher[row * entries + k]) : -INFINITY;
-    student[k] = used ? to_f32(x[j]) : 0.0f;
-    t = merge(t, peak_sum_t { p[k], p[k] == -INFINITY ? 0.0f :
-      (isnan(p[k]) ? p[k] : 1.0f) }, c);
+    p[k] = logit;
+    student[k] = used && (!rank || own((int)j)) ? to_f32(x[j]) : 0.0f;
+    t = merge(t, peak_sum_t { logit, logit == -INFINITY ? 0.0f :
+      isnan(logit) ? logit : 1.0f }, c);
   }
-  t = cta_merge<nt>(t, c, merged);
+  t = warp_merge(t, c);
+  if(!lane) teacher_part[warp] = t;
+
+  // One pass over the student's logits.
+  float peak = edge_value;
+  #pragma unroll
+  for(int i = 0; i < held; ++i)
+    #pragma unroll
+    for(int j = 0; j < pack; ++j) peak = fmaxf(peak, to_f32(word[i].v[j]));
+  float base = peak == -INFINITY ? 0.0f : peak, sum = 0;
+  #pragma unroll
+  for(int i = 0; i < held; ++i)
+    #pragma unroll
+    for(int j = 0; j < pack; ++j)
+      sum += exp2_fast((to_f32(word[i].v[j]) - base) * c);
+  sum += exp2_fast((edge_value - base) * c);
+  peak_sum_t s { peak, sum };
+  for(int w = begin + held * nt + tid; w < end; w += nt) {
+    word_t more = x_words[w];
+    peak = s.peak;
+    #pragma unroll
+    for(int j = 0; j < pack; ++j) peak = fmaxf(peak, to_f32(more.v[j]));
+    base = peak == -INFINITY ? 0.0f : peak;
+    sum = s.sum * exp2_fast((s.peak - base) * c);
+    #pragma unroll
+    for(int j = 0; j < pack; ++j)
+      sum += exp2_fast((to_f32(more.v[j]) - base) * c);
+    s = peak_sum_t { peak, sum };
+  }
+  s = warp_merge(s, c);
+  if(1 == ctas) {
+    if(!lane) part[warp] = s;
+    __syncthreads();
+  } else {
+    ptx::cluster_wait();                     // every CTA has started
+    if(lane < ctas)
+      cluster.map_shared_rank(part, lane)[rank * warps + warp] = s;
+    cluster.sync();
+  }
+  s = peak_sum_t { -INFINITY, 0.0f };
+  #pragma unroll
+  for(int i = 0; i < parts / 32; ++i) {
+    int q = i * 32 + lane;
+    if(q < ctas * warps) s = merge(s, part[q], c);
+  }
+  s = warp_merge(s, c);
+  t = warp_merge(lane < warps ? teacher_part[lane] :
+    peak_sum_t { -INFINITY, 0.0f }, c);
   bool taught = t.peak > -INFINITY || isnan(t.sum);
-  if(taught) {
-    float log_sum = logf(t.sum);
-    // One pass over the student's logits.
-    peak_sum_t s { -INFINITY, 0.0f };
-    for(int v = tid * pack; v < vocabulary; v += nt * pack) {
-      word_t word = *(const word_t*)(x + v);
-      float peak = s.peak;
-      #pragma unroll
-      for(int j = 0; j < pack; ++j) peak = fmaxf(peak, to_f32(word.v[j]));
-      float base = peak == -INFINITY ? 0.0f : peak;
-      float sum = s.sum * exp2_fast((s.peak - base) * c);
-      #pragma unroll
-      for(int j = 0; j < pack; ++j)
-        sum += exp2_fast((to_f32(word.v[j]) - base) * c);
-      s = peak_sum_t { peak, sum };
-    }
-    s = cta_merge<nt>(s, c, merged);
-    bool empty = s.peak == -INFINITY && !isnan(s.sum);
-    float loss = 0;
-    float log_mass = logf(s.sum);
-    for(int k = tid; k < entries; k += nt) {
-      float log_p = (p[k] - t.peak) / temperature - log_sum;
-      float prob = at[k] < 0 ? 0.0f : expf(log_p);
+  bool none = !taught || (s.peak == -INFINITY && !isnan(s.sum));
+
+  // From logits to probabilities, and the first CTA adds up the loss.
+  float log_sum = logf(t.sum), log_mass = logf(s.sum), loss = 0;
+  for(int k = tid; k < entries; k += nt) {
+    float log_p = (p[k] - t.peak) / temperature - log_sum;
+    float prob = at[k] < 0 ? 0.0f : expf(log_p);
+    if(!rank && prob != 0 && !none) {
       float log_q = (student[k] - s.peak) / temperature - log_mass;
-      if(prob != 0) loss += prob * (log_p - log_q);
-      p[k] = prob;
+      loss += prob * (log_p - log_q);
     }
-    loss = cta_sum<nt>(loss, summed);
-    if(!tid) losses[row] = empty ? 0.0f : temperature * temperature * loss;
-    if(want_grad) {
-      real_t* g = grad + row * grad_stride;
-      float factor = weight * temperature / s.sum;
-      for(int v = tid * pack; v < vocabulary; v += nt * pack) {
-        word_t word = *(const word_t*)(x + v);
+    p[k] = prob;
+  }
+  if(!rank) {
+    #pragma unroll
+    for(int offset = 16; offset; offset /= 2)
+      loss += __shfl_xor_sync(0xffffffffu, loss, offset);
+    if(!lane) loss_part[warp] = loss;
+    __syncthreads();
+    if(!tid) {
+      loss = 0;
+      for(int w = 0; w < warps; ++w) loss += loss_part[w];
+      losses[row] = none ? 0.0f : temperature * temperature * loss;
+    }
+  }
+  if(want_grad) {
+    float factor = weight * temperature / s.sum;
+    auto slope = [&](float value) {
+      return none ? 0.0f : factor * exp2_fast((value - s.peak) * c);
+    };
+    word_t* g_words = (word_t*)(g + head);
+    #pragma unroll
+    for(int i = 0; i < held; ++i) {
+      int w = begin + i * nt + tid;
+      if(w < end) {
         #pragma unroll
         for(int j = 0; j < pack; ++j)
-          word.v[j] = from_f32<real_t>(empty ? 0.0f : factor *
-            exp2_fast((to_f32(word.v[j]) - s.peak) * c));
-        *(word_t*)(g + v) = word;
-      }
-      __syncthreads();
-      // The teacher's tokens again, each with all of its entries.
-      for(int k = tid; k < entries; k += nt) {
-        if(at[k] < 0 || empty) continue;
-        float sum = 0;
-        for(int i = 0; i < entries; ++i)
-          if(at[i] == at[k]) sum += p[i];
-        g[at[k]] = from_f32<real_t>(factor *
-          exp2_fast((student[k] - s.peak) * c) - weight * temperature * sum);
+          word[i].v[j] = from_f32<real_t>(slope(to_f32(word[i].v[j])));
+        store_streaming(g_words + w, word[i]);
       }
     }
-  } else {
-    if(!tid) losses[row] = 0.0f;
-    if(want_grad) {
-      word_t word;
+    for(int w = begin + held * nt + tid; w < end; w += nt) {
+      word_t more = x_words[w];
       #pragma unroll
-      for(int j = 0; j < pack; ++j) word.v[j] = from_f32<real_t>(0.0f);
-      for(int v = tid * pack; v < vocabulary; v += nt * pack)
-        *(word_t*)(grad + row * grad_stride + v) = word;
+      for(int j = 0; j < pack; ++j)
+        more.v[j] = from_f32<real_t>(slope(to_f32(more.v[j])));
+      store_streaming(g_words + w, more);
     }
+    if(edge >= 0) g[edge] = from_f32<real_t>(slope(edge_value));
+    __syncthreads();
+    // The teacher's tokens in this CTA's part again, each with all of its
+    // entries.
+    for(int k = tid; k < entries && !none; k += nt) {
+      if(at[k] < 0 || !own(at[k])) continue;
+      float taken = 0;
+      for(int i = 0; i < entries; ++i)
+        if(at[i] == at[k]) taken += p[i];
+      g[at[k]] = from_f32<real_t>(slope(student[k]) -
+        weight * temperature * taken);
+    }
+  }
+}
+
+// The rows stream through a ring of landing buffers that one thread keeps filled
+// by bulk copies, without a pause between rows: each row (or a CTA's part of it)
+// passes once for its peak and mass and, with want_grad, at once again for the
+// gradient, this time from the L2 (a row for each SM takes 40 MB of it at 2^17
+// logits of 16 bits). HBM sees one read, and one write, of the logits.
+//
+// nt threads take the words; a warp of its own starts the copies, and another one
+// is a row ahead with the teacher: it reduces the entries to what the CTA needs
+// of them, the list of tokens in its part with their probabilities and the
+// student's logits, and of p and p (s - the greatest of these logits) the sums,
+// which is all that the loss needs: log q_j = (s_j - peak) / T - log mass.
+enum { distill_words = 4 };        // a thread's words in a landing buffer
+
+#ifndef DOCC
+#define DOCC 4
+#endif
+struct distill_list_t {
+  int listed, taught;
+  float weight, entropy;           // entropy: sum of p log p over all entries
+  float share, product, from;
+};
+
+template<int nt>
+struct distill_shared_t {
+  enum { warps = nt / 32, most_stages = 8 };
+  uint64_t full[most_stages], empty[most_stages];
+  uint64_t list_full[2], list_empty[2];
+  uint64_t told[2];
+  distill_list_t list[2];
+  peak_sum_t part[2][warps];
+  float4 news[2][distill_max_cluster];         // peak, sum, share, product
+  float news_from[2][distill_max_cluster];
+};
+// Behind the landing buffers, for each entry: two lists of {token, p, p of all
+// entries with the token, student's logit} and the teacher's own scratch.
+enum { distill_entry_bytes = 2 * 16 + 8 };
+
+// Two neighbouring values as a pair of floats, and back with one rounding.
+MGPU_DEVICE __forceinline__ uint64_t two_values(const float* v) {
+  return ptx::make_pair(v[0], v[1]);
+}
+MGPU_DEVICE __forceinline__ uint64_t two_values(const __nv_bfloat16* v) {
+  uint32_t bits;
+  memcpy(&bits, v, 4);
+  return ptx::make_pair(__uint_as_float(bits << 16),
+    __uint_as_float(bits & 0xffff0000u));
+}
+MGPU_DEVICE __forceinline__ uint64_t two_values(const __half* v) {
+  __half2 two;
+  memcpy(&two, v, 4);
+  float2 f = __half22float2(two);
+  return ptx::make_pair(f.x, f.y);
+}
+MGPU_DEVICE __forceinline__ void store_two(float* v, float2 f) {
+  v[0] = f.x;
+  v[1] = f.y;
+}
+MGPU_DEVICE __forceinline__ void store_two(__nv_bfloat16* v, float2 f) {
+  __nv_bfloat162 two = __floats2bfloat162_rn(f.x, f.y);
+  memcpy(v, &two, 4);
+}
+MGPU_DEVICE __forceinline__ void store_two(__half* v, float2 f) {
+  __half2 two = __floats2half2_rn(f.x, f.y);
+  memcpy(v, &two, 4);
+}
+
+// The greatest of a thread's words (a NaN only where there is nothing else).
+template<int held, int pack>
+MGPU_DEVICE __forceinline__ float words_peak(
+  const pack_t<float, pack> (&word)[held]) {
+  float peak = -INFINITY;
+  #pragma unroll
+  for(int i = 0; i < held; ++i)
+    #pragma unroll
+    for(int j = 0; j < pack; ++j) peak = fmaxf(peak, word[i].v[j]);
+  return peak;
+}
+template<typename pair_t, typename real_t, int held, int pack>
+MGPU_DEVICE __forceinline__ float pairs_peak(
+  const pack_t<real_t, pack> (&word)[held]) {
+  pair_t peak;
+  memcpy(&peak, &word[0].v[0], 4);
+  #pragma unroll
+  for(int i = 0; i < held; ++i)
+    #pragma unroll
+    for(int j = 0; j < pack; j += 2) {
+      pair_t two;
+      memcpy(&two, &word[i].v[j], 4);
+      peak = __hmax2(peak, two);
+    }
+  return fmaxf(to_f32(peak.x), to_f32(peak.y));
+}
+template<int held, int pack>
+MGPU_DEVICE __forceinline__ float words_peak(
+  const pack_t<__half, pack> (&word)[held]) {
+  return pairs_peak<__half2>(word);
+}
+template<int held, int pack>
+MGPU_DEVICE __forceinline__ float words_peak(
+  const pack_t<__nv_bfloat16, pack> (&word)[held]) {
+  return pairs_peak<__nv_bfloat162>(word);
+}
+
+template<int nt, int pack, bool want_grad, typename real_t>
+__global__ void __launch_bounds__(nt + 64, nt == 512 ? 1 : DOCC)
+distill_stream_k(const real_t* logits, int64_t stride, int count,
+  int vocabulary, int log_ctas, int stages, distill_teacher_t teacher,
+  float temperature, const float* weights, float* losses, real_t* grad,
+  int64_t grad_stride, uint64_t timeout_ns) {
+  typedef pack_t<real_t, pack> word_t;
+  typedef distill_shared_t<nt> shared_t;
+  enum { warps = nt / 32, held = distill_words, chunk = nt * held };
+  extern __shared__ __align__(128) char memory[];
+  __shared__ shared_t shared;
+
+  const int entries = teacher.entries, ctas = 1 << log_ctas;
+  word_t* buffers = (word_t*)memory;
+  float4* lists = (float4*)(memory + (size_t)stages * chunk * 16);
+  int tid = (int)threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int rank = (int)blockIdx.x & (ctas - 1);
+  int clusters = (int)gridDim.x >> log_ctas;
+  const float c = 1.4426950408889634f / temperature;
+  const float per_t = 1.0f / temperature;
+
+  if(!tid) {
+    for(int i = 0; i < stages; ++i) {
+      ptx::mbar_init(&shared.full[i], 1);
+      ptx::mbar_init(&shared.empty[i], warps);
+    }
+    for(int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&shared.list_full[i], 1);
+      ptx::mbar_init(&shared.list_empty[i], warps);
+      ptx::mbar_init(&shared.told[i], 1);
+    }
+    ptx::fence_mbar_init_cluster();
+    ptx::fence_proxy_async();
+  }
+  if(ctas > 1) cooperative_groups::this_cluster().sync();
+  else __syncthreads();
+
+  // A row's whole words between its 16-byte borders, and this CTA's part: words
+  // [begin, end). The elements outside are the first CTA's.
+  int head, words, begin, end;
+  auto cut = [&](const real_t* x) {
+    head = min((int)((16 - (uintptr_t)x % 16) % 16 / sizeof(real_t)) % pack,
+      vocabulary);
+    words = (vocabulary - head) / pack;
+    int per_cta = (words + ctas - 1) >> log_ctas;
+    begin = min(rank * per_cta, words);
+    end = min(begin + per_cta, words);
+  };
+  int64_t row = (int64_t)blockIdx.x >> log_ctas;
+  int stage = 0;
+  uint32_t parity = 0;
+  auto next_stage = [&]() {
+    if(++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  };
+
+  if(warp == warps) {
+    // The copies.
+    if(lane) return;
+    for(; row < count; row += clusters) {
+      const real_t* x = logits + row * stride;
+      cut(x);
+      const word_t* from = (const word_t*)(x + head);
+      #pragma unroll 1
+      for(int pass = 0; pass < (want_grad ? 2 : 1); ++pass)
+        for(int w = begin; w < end; w += chunk) {
+          // The first round finds the buffers empty.
+          if(!ptx::mbar_wait(&shared.empty[stage], parity ^ 1, timeout_ns))
+            return;
+          uint32_t bytes = (uint32_t)min((int)chunk, end - w) * 16;
+          ptx::mbar_arrive_expect_tx(&shared.full[stage], bytes);
+          ptx::bulk_load(buffers + stage * chunk, from + w, bytes,
+            &shared.full[stage]);
+          next_stage();
+        }
+    }
+    return;
+  }
+  if(warp == warps + 1) {
+    // The teacher.
+    float* logit = (float*)(lists + 2 * entries);
+    int* token = (int*)(logit + entries);
+    // Entries on their way: the first ones of the next row already while this
+    // one's are reduced.
+    enum { batch = 4 };
+    int64_t next_token[batch];
+    float next_logit[batch], next_weight = 1.0f;
+    auto request = [&](int64_t r, int first) {
+      #pragma unroll
+      for(int b = 0; b < batch; ++b) {
+        int64_t k = first + b * 32 + lane;
+        next_token[b] = k < entries ? teacher.token(r * entries + k) : -1;
+        next_logit[b] = k < entries ? teacher.logit(r * entries + k) : 0.0f;
+      }
+      if(weights && !first) next_weight = weights[r];
+    };
+    if(row < count) request(row, 0);
+    for(int turn = 0; row < count; ++turn, row += clusters) {
+      int set = turn & 1;
+      const real_t* x = logits + row * stride;
+      cut(x);
+      if(!ptx::mbar_wait(&shared.list_empty[set], (uint32_t)(turn >> 1 & 1) ^ 1,
+        timeout_ns)) return;
+      float weight = next_weight;
+      float peak = -INFINITY, sum = 0;
+      for(int first = 0; first < entries; first += batch * 32) {
+        if(first) request(row, first);
+        #pragma unroll
+        for(int b = 0; b < batch; ++b) {
+          int k = first + b * 32 + lane;
+          bool used = next_token[b] >= 0 && next_token[b] < vocabulary &&
+            weight != 0;
+          if(k < entries) {
+            token[k] = used ? (int)next_token[b] : -1;
+            logit[k] = used ? next_logit[b] : -INFINITY;
+          }
+          if(used) peak = fmaxf(peak, next_logit[b]);
+        }
+      }
+      if(row + clusters < count) request(row + clusters, 0);
+      #pragma unroll
+      for(int offset = 16; offset; offset /= 2)
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, offset));
+      // A NaN stays one.
+      for(int k = lane; k < entries; k += 32)
+        if(logit[k] != -INFINITY) sum += expf((logit[k] - peak) * per_t);
+      #pragma unroll
+      for(int offset = 16; offset; offset /= 2)
+        sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+      bool taught = peak > -INFINITY || isnan(sum);
+      float log_sum = logf(sum), entropy = 0, from = -INFINITY;
+      float4* list = lists + set * entries;
+      int listed = 0;
+      for(int first = 0; first < entries; first += 32) {
+        int k = first + lane;
+        float prob = 0;
+        int j = -1;
+        if(k < entries && taught && logit[k] != -INFINITY) {
+          float log_p = (logit[k] - peak) * per_t - log_sum;
+          prob = expf(log_p);
+          if(prob != 0) {
+            entropy += prob * log_p;
+            j = token[k];
+          }
+        }
+        int w = j < head ? -1 : (j - head) / pack;
+        bool own = j >= 0 && (w < 0 || w >= words ? !rank :
+          w >= begin && w < end);
+        unsigned votes = __ballot_sync(0xffffffffu, own);
+        if(own) list[listed + __popc(votes & ((1u << lane) - 1))] =
+          make_float4(__int_as_float(j), prob, prob, 0.0f);
+        listed += __popc(votes);
+      }
+      __syncwarp();
+      // The student's logits: read before anybody waits for the list, which comes
+      // before the gradient is written, perhaps in their place.
+      #pragma unroll 4
+      for(int i = lane; i < listed; i += 32) {
+        float value = to_f32(x[__float_as_int(list[i].x)]);
+        list[i].w = value;
+        from = fmaxf(from, value);
+      }
+      #pragma unroll
+      for(int offset = 16; offset; offset /= 2)
+        from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, offset));
+      if(from == -INFINITY) from = 0;
+      float share = 0, product = 0;
+      for(int i = lane; i < listed; i += 32) {
+        float4 mine = list[i];
+        share += mine.y;
+        product += mine.y * (mine.w - from);
+        if(want_grad) {
+          // All of a token's entries together.
+          float taken = 0;
+          #pragma unroll 4
+          for(int q = 0; q < listed; ++q) {
+            float4 other = list[q];
+            if(__float_as_int(other.x) == __float_as_int(mine.x))
+              taken += other.y;
+          }
+          list[i].z = taken;
+        }
+      }
+      #pragma unroll
+      for(int offset = 16; offset; offset /= 2) {
+        entropy += __shfl_xor_sync(0xffffffffu, entropy, offset);
+        share += __shfl_xor_sync(0xffffffffu, share, offset);
+        product += __shfl_xor_sync(0xffffffffu, product, offset);
+      }
+      if(!lane) shared.list[set] = distill_list_t { listed, (int)taught, weight,
+        entropy, share, product, from };
+      __syncwarp();
+      if(!lane) ptx::mbar_arrive(&shared.list_full[set]);
+    }
+    return;
+  }
+
+  bool good = true;
+  auto take = [&](word_t (&word)[held], int here) {
+    good = good && ptx::mbar_wait(&shared.full[stage], parity, timeout_ns);
+    const word_t* buffer = buffers + stage * chunk;
+    #pragma unroll
+    for(int i = 0; i < held; ++i) {
+      int w = i * nt + tid;
+      if(w < here) word[i] = buffer[w];
+      else {
+        #pragma unroll
+        for(int j = 0; j < pack; ++j)
+          word[i].v[j] = from_f32<real_t>(-INFINITY);
+      }
+    }
+    __syncwarp();
+    if(!lane) ptx::mbar_arrive(&shared.empty[stage]);
+    next_stage();
+  };
+  const uint64_t c_pair = ptx::make_pair(c, c);
+  for(int turn = 0; row < count; ++turn, row += clusters) {
+    int set = turn & 1;
+    const real_t* x = logits + row * stride;
+    cut(x);
+    int tail = vocabulary - head - words * pack;
+    int edge = rank ? -1 : tid < head ? tid :
+      tid < head + tail ? vocabulary - tail + (tid - head) : -1;
+    float edge_value = edge >= 0 ? to_f32(x[edge]) : -INFINITY;
+
+    // The first pass: weights relative to the thread's peak so far.
+    float peak = -INFINITY;
+    uint64_t sums = 0;
+    #pragma unroll 1
+    for(int w = begin; w < end; w += chunk) {
+      word_t word[held];
+      take(word, end - w);
+      float higher = fmaxf(peak, words_peak(word));
+      float base = higher == -INFINITY ? 0.0f : higher;
+      if(higher > peak) {
+        float scale = exp2_fast((peak - base) * c);
+        sums = ptx::mul_pair(sums, ptx::make_pair(scale, scale));
+        peak = higher;
+      }
+      const uint64_t minus_base = ptx::make_pair(-base, -base);
+      #pragma unroll
+      for(int i = 0; i < held; ++i)
+        #pragma unroll
+        for(int j = 0; j < pack; j += 2) {
+          float2 power = ptx::pair_values(ptx::mul_pair(ptx::add_pair(
+            two_values(&word[i].v[j]), minus_base), c_pair));
+          sums = ptx::add_pair(sums, ptx::make_pair(exp2_fast(power.x),
+            exp2_fast(power.y)));
+        }
+    }
+    peak_sum_t s { peak, ptx::pair_values(sums).x + ptx::pair_values(sums).y };
+    s = merge(s, peak_sum_t { edge_value, edge_value == -INFINITY ? 0.0f :
+      isnan(edge_value) || edge_value == INFINITY ? NAN : 1.0f }, c);
+    s = warp_merge(s, c);
+    if(!lane) shared.part[set][warp] = s;
+    ptx::named_sync<1, nt>();
+    s = warp_merge(lane < warps ? shared.part[set][lane] :
+      peak_sum_t { -INFINITY, 0.0f }, c);
+
+    good = good && ptx::mbar_wait(&shared.list_full[set],
+      (uint32_t)(turn >> 1 & 1), timeout_ns);
+    distill_list_t list = shared.list[set];
+    float share = list.share, distance = list.product;
+    if(ctas > 1) {
+      // Two sets of slots and barriers: a CTA sends the news of the turn after
+      // the next only when it has this CTA's of the next, which are sent behind
+      // the wait for those of this turn.
+      if(!warp) {
+        if(!lane) ptx::mbar_arrive_expect_tx(&shared.told[set],
+          (uint32_t)ctas * 20);
+        if(lane < ctas) {
+          uint32_t bar = ptx::cluster_addr(&shared.told[set], lane);
+          ptx::store_async(ptx::cluster_addr(&shared.news[set][rank], lane),
+            s.peak, s.sum, list.share, list.product, bar);
+          ptx::store_async(ptx::cluster_addr(&shared.news_from[set][rank], lane),
+            list.from, bar);
+        }
+      }
+      good = good && ptx::mbar_wait(&shared.told[set],
+        (uint32_t)(turn >> 1 & 1), timeout_ns);
+      float4 n = lane < ctas ? shared.news[set][lane] :
+        make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+      s = warp_merge(peak_sum_t { n.x, n.y }, c);
+    }
+    float base = s.peak == -INFINITY ? 0.0f : s.peak, mass = s.sum;
+    if(!good) {                              // a wait ran out: no result
+      mass = NAN;
+      list.taught = 1;
+      list.listed = 0;
+      if(!lane) raise_status(nullptr, (uint32_t)status_copy_timeout);
+    }
+    bool none = !list.taught || (s.peak == -INFINITY && !isnan(mass));
+    if(!rank && !tid) {
+      float to_peak = 0;
+      if(1 == ctas) {
+        if(share != 0) to_peak = distance + share * (list.from - base);
+      } else {
+        share = 0;
+        for(int r = 0; r < ctas; ++r) {
+          float4 n = shared.news[set][r];
+          share += n.z;
+          if(n.z != 0) to_peak += n.w + n.z * (shared.news_from[set][r] - base);
+        }
+      }
+      float loss = list.entropy + share * logf(mass) - to_peak * per_t;
+      losses[row] = none ? 0.0f : temperature * temperature * loss;
+    }
+
+    if(want_grad) {
+      float factor = none ? 0.0f : list.weight * temperature / mass;
+      real_t* g = grad + row * grad_stride;
+      word_t* g_words = (word_t*)(g + head);
+      const uint64_t minus_base = ptx::make_pair(-base, -base);
+      const uint64_t factor_pair = ptx::make_pair(factor, factor);
+      #pragma unroll 1
+      for(int w = begin; w < end; w += chunk) {
+        word_t word[held];
+        take(word, end - w);
+        #pragma unroll
+        for(int i = 0; i < held; ++i) {
+          #pragma unroll
+          for(int j = 0; j < pack; j += 2) {
+            float2 power = ptx::pair_values(ptx::mul_pair(ptx::add_pair(
+              two_values(&word[i].v[j]), minus_base), c_pair));
+            store_two(&word[i].v[j], ptx::pair_values(ptx::mul_pair(
+              ptx::make_pair(exp2_fast(power.x), exp2_fast(power.y)),
+              factor_pair)));
+          }
+          // A row without a gradient: 0, even where a logit is not a number.
+          if(none) word[i] = word_t();
+          int at = w + i * nt + tid;
+          if(at < end) store_streaming(g_words + at, word[i]);
+        }
+      }
+      if(edge >= 0) g[edge] = from_f32<real_t>(none ? 0.0f :
+        factor * exp2_fast((edge_value - base) * c));
+      // Then the teacher's tokens in this CTA's part again.
+      ptx::named_sync<1, nt>();
+      const float4* entry = lists + set * entries;
+      for(int i = tid; i < list.listed && !none; i += nt)
+        g[__float_as_int(entry[i].x)] = from_f32<real_t>(factor *
+          exp2_fast((entry[i].w - base) * c) -
+          list.weight * temperature * entry[i].z);
+    }
+    __syncwarp();
+    if(!lane) ptx::mbar_arrive(&shared.list_empty[set]);
   }
 }
 
@@ -179,26 +728,72 @@ template<bool want_grad, typename real_t, typename teacher_t, typename token_t>
 void distill_enqueue(const real_t* logits, int64_t stride, int count,
   int vocabulary, const token_t* tokens, const teacher_t* teacher, int entries,
   float temperature, const float* weights, float* losses, real_t* grad,
-  int64_t grad_stride, cudaStream_t stream) {
+  int64_t grad_stride, cudaStream_t stream,
+  uint64_t timeout_ns = 2000000000ull) {
   if(!count) return;
-  int pack = pack_limit(logits, stride, vocabulary, (int)sizeof(real_t));
-  if(want_grad)
-    pack = min(pack, pack_limit(grad, grad_stride, vocabulary,
-      (int)sizeof(real_t)));
-  auto launch = [&](auto tag) {
-    enum { nt = 512 };
-    distill_k<nt, decltype(tag)::value, want_grad, real_t, teacher_t, token_t>
-      <<<(unsigned)count, nt, 0, stream>>>(logits, stride, vocabulary, tokens,
-        teacher, entries, temperature, weights, losses, grad, grad_stride);
-  };
-  switch(pack) {
-    case 8: launch(std::integral_constant<int,
-      (sizeof(real_t) == 2 ? 8 : 4)>()); break;
-    case 4: launch(std::integral_constant<int, 4>()); break;
-    case 2: launch(std::integral_constant<int, 2>()); break;
-    default: launch(std::integral_constant<int, 1>()); break;
+  enum { size = sizeof(real_t) };
+  // Words of 16 bytes where rows of the logits and of the gradient begin at the
+  // same place of one.
+  bool apart = want_grad && ((uintptr_t)logits % 16 != (uintptr_t)grad % 16 ||
+    (count > 1 && (stride - grad_stride) * size % 16));
+  int64_t row_bytes = (int64_t)vocabulary * size;
+  distill_teacher_t source { tokens, teacher, sizeof(token_t) == 8,
+    teacher_kind(teacher), entries };
+  cudaLaunchConfig_t config = { };
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  if(apart) {
+    enum { nt = 256 };
+    int ctas = 1;
+    while(ctas < distill_max_cluster && (int64_t)count * ctas < 296 &&
+      vocabulary / ctas > 4096) ctas *= 2;
+    config.gridDim = dim3((unsigned)((int64_t)count * ctas));
+    config.blockDim = dim3(nt);
+    config.dynamicSmemBytes = 12 * (size_t)entries;
+    attribute.val.clusterDim.x = (unsigned)ctas;
+    throw_on_error(cudaLaunchKernelEx(&config,
+      distill_k<nt, 1, want_grad, real_t>, logits, stride, vocabulary, ctas,
+      source, temperature, weights, losses, grad, grad_stride));
+    return;
   }
-  throw_on_error(cudaGetLastError());
+#ifndef DSMALL
+#define DSMALL (96 << 10)
+#endif
+#ifndef DC
+#define DC 0
+#endif
+  auto launch = [&](auto threads) {
+    enum { nt = decltype(threads)::value, per_sm = nt == 512 ? 1 : DOCC,
+      stage_bytes = nt * distill_words * 16 };
+    auto kernel = distill_stream_k<nt, 16 / (int)size, want_grad, real_t>;
+    // What an SM has, less the shared variables of fixed size.
+    const int room = (224 << 10) / per_sm - 2048;
+    int lists = distill_entry_bytes * entries;
+    int stages = (room - lists) / stage_bytes;
+    stages = stages < 3 ? 3 : stages > 6 ? 6 : stages;
+    set_dynamic_smem<decltype(threads), std::integral_constant<bool, want_grad>,
+      real_t>(kernel, 224 << 10);
+    // Clusters where there are too few rows for all SMs, or for whole rounds of
+    // them.
+    int slots = 148 * per_sm, ctas = 1;
+    while(ctas < distill_max_cluster && row_bytes / ctas > 2 * stage_bytes &&
+      (int64_t)count * ctas < 6 * slots) ctas *= 2;
+    if(DC) ctas = DC;
+    int log_ctas = ctas < 2 ? 0 : ctas < 4 ? 1 : ctas < 8 ? 2 : 3;
+    attribute.val.clusterDim.x = (unsigned)ctas;
+    config.blockDim = dim3(nt + 64);
+    config.dynamicSmemBytes = (size_t)stages * stage_bytes + lists;
+    config.gridDim = dim3((unsigned)(min(count, slots / ctas) * ctas));
+    throw_on_error(cudaLaunchKernelEx(&config, kernel, logits, stride, count,
+      vocabulary, log_ctas, stages, source, temperature, weights, losses, grad,
+      grad_stride, timeout_ns));
+  };
+  if(row_bytes > DSMALL) launch(std::integral_constant<int, 512>());
+  else launch(std::integral_constant<int, 128>());
 }
 
 } // namespace detail

@@ -263,6 +263,7 @@ token_cluster_sort_k(token_keys_t<token_t> source, int count, int bits,
   typedef token_cluster_shared_t<vt> shared_t;
   shared_t& shared = *(shared_t*)token_cluster_memory;
   auto cluster = cooperative_groups::this_cluster();
+  ptx::cluster_arrive_relaxed();
   // The kernel that follows zeroes the rows without a token meanwhile.
   ptx::grid_launch_dependents();
 
@@ -306,6 +307,7 @@ token_cluster_sort_k(token_keys_t<token_t> source, int count, int bits,
       }
     }
     __syncthreads();
+    if(!pass) ptx::cluster_wait();           // every CTA has started
     // Two digits to a thread, in the halves of a word: the warps' counts become
     // places in the CTA, and every CTA is told the CTA's totals.
     if(tid * 2 < digits) {

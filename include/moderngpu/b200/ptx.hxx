@@ -214,6 +214,30 @@ __device__ __forceinline__ type_t ld_no_l1_hint(const type_t* p, uint64_t policy
 }
 
 ////////////////////////////////////////////////////////////////////////////////
+// Two 32-bit floats in one register pair: one instruction for both.
+
+__device__ __forceinline__ uint64_t make_pair(float lo, float hi) {
+  uint64_t pair;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(pair) : "f"(lo), "f"(hi));
+  return pair;
+}
+__device__ __forceinline__ float2 pair_values(uint64_t pair) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(pair));
+  return v;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+////////////////////////////////////////////////////////////////////////////////
 // Named barrier over `count` threads (a multiple of 32) of the CTA.
 
 template<int id, int count>
@@ -236,6 +260,46 @@ __device__ __forceinline__ bool named_all(bool mine) {
     "}\n"
     : "=r"(out) : "r"((uint32_t)mine), "n"(id), "n"(count) : "memory");
   return out != 0;
+}
+
+////////////////////////////////////////////////////////////////////////////////
+// Barrier over all threads of a cluster, in two halves. Shared memory of another
+// CTA may be touched only once that CTA has started: a kernel arrives when it
+// begins and waits before its first remote access. The relaxed arrival orders
+// no memory; later barriers are cooperative_groups' cluster.sync().
+
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The address of a variable of this CTA's shared memory in another CTA of the
+// cluster, and a store of 16 or 4 bytes there that counts its bytes on an
+// mbarrier of the same CTA. Unlike a barrier of the cluster, whose arrival is a
+// release, it does not wait for the thread's earlier stores to global memory.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there)
+    : "r"(smem_addr(p)), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void store_async(uint32_t to, float a, float b,
+  float c, float d, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 "
+    "[%0], {%1, %2, %3, %4}, [%5];"
+    :: "r"(to), "f"(a), "f"(b), "f"(c), "f"(d), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void store_async(uint32_t to, float a,
+  uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 "
+    "[%0], %1, [%2];" :: "r"(to), "f"(a), "r"(bar) : "memory");
+}
+// Makes the initialisation of mbarriers visible to the cluster's other CTAs
+// (with a barrier of the cluster behind it).
+__device__ __forceinline__ void fence_mbar_init_cluster() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
 ////////////////////////////////////////////////////////////////////////////////

@@ -18,6 +18,7 @@
 #pragma once
 #include "runtime.hxx"
 #include "real_types.hxx"
+#include "ptx.hxx"
 #ifdef __CUDACC__
 #include <cooperative_groups.h>
 #endif
@@ -254,6 +255,7 @@ struct sample_cta_t {
     });
     sample_news_t mine = { };
     mine.p = fold_max(key);
+    ptx::cluster_wait();                     // every CTA has started
     const sample_news_t* news = share(mine);
     key = 0;
     for(int r = 0; r < ctas; ++r) key = max(key, news[r].p);
@@ -801,6 +803,7 @@ __global__ void __launch_bounds__(nt)
 sample_k(const real_t* logits, int64_t stride, int vocabulary,
   const float* uniforms, sampling_t settings, int* tokens, int ctas) {
   __shared__ sample_shared_t<nt> shared;
+  ptx::cluster_arrive_relaxed();
   int64_t at = (int64_t)blockIdx.x / ctas;
   float temperature = settings.temperatures ? settings.temperatures[at] :
     settings.temperature;
