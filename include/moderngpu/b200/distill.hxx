@@ -82,191 +82,94 @@ inline int teacher_kind(const float*) { return 0; }
 inline int teacher_kind(const __half*) { return 1; }
 inline int teacher_kind(const __nv_bfloat16*) { return 2; }
 
-// A cluster of CTAs per row, each with a part of it. The first `held` words of
-// 16 bytes of each thread are requested at once and stay in registers, so that a
-// row which fits (32 KB a CTA) is read once and its gradient written from there;
-// what goes beyond is read again, from the L2. Bound by HBM bytes: one read, and
-// with want_grad one write, of the logits. The only exchange is one of a peak
-// and a sum for each warp.
-template<int nt, int pack, bool want_grad, typename real_t>
-__global__ void __launch_bounds__(nt, 768 / nt)
-distill_k(const real_t* logits, int64_t stride, int vocabulary, int ctas,
+// Rows of the logits and of the gradient that begin at different places of a
+// 16-byte word: one CTA to a row, element by element, the second pass from the
+// L2.
+template<int nt, typename real_t>
+__global__ void __launch_bounds__(nt)
+distill_apart_k(const real_t* logits, int64_t stride, int vocabulary,
   distill_teacher_t teacher, float temperature, const float* weights,
   float* losses, real_t* grad, int64_t grad_stride) {
-  typedef pack_t<real_t, pack> word_t;
-  enum { warps = nt / 32, held = 8, parts = distill_max_cluster * warps };
+  enum { warps = nt / 32 };
   extern __shared__ int distill_memory[];
-  __shared__ peak_sum_t part[parts];
-  __shared__ peak_sum_t teacher_part[warps];
+  __shared__ peak_sum_t part[warps], teacher_part[warps];
   __shared__ float loss_part[warps];
-  auto cluster = cooperative_groups::this_cluster();
-  if(ctas > 1) ptx::cluster_arrive_relaxed();
-
   int entries = teacher.entries;
   int* at = distill_memory;                  // -1: unused
   float* p = (float*)(distill_memory + entries);
   float* student = p + entries;
   int tid = (int)threadIdx.x, lane = tid % 32, warp = tid / 32;
-  int rank = (int)blockIdx.x % ctas;
-  int64_t row = (int64_t)blockIdx.x / ctas;
+  int64_t row = blockIdx.x;
   const real_t* x = logits + row * stride;
   real_t* g = grad + row * grad_stride;
   const float c = 1.4426950408889634f / temperature;
-
-  // Whole words between the row's first and last 16-byte border, an equal part
-  // of them for each CTA; the elements outside, one to a thread of the first.
-  int head = min((int)((16 - (uintptr_t)x % 16) % 16 / sizeof(real_t)) % pack,
-    vocabulary);
-  int words = (vocabulary - head) / pack;
-  int tail = vocabulary - head - words * pack;
-  const word_t* x_words = (const word_t*)(x + head);
-  int per_cta = div_up(words, ctas);
-  int begin = min(rank * per_cta, words), end = min(begin + per_cta, words);
-  int edge = rank ? -1 : tid < head ? tid :
-    tid < head + tail ? vocabulary - tail + (tid - head) : -1;
-
-  word_t word[held];
-  #pragma unroll
-  for(int i = 0; i < held; ++i) {
-    int w = begin + i * nt + tid;
-    if(w < end) word[i] = x_words[w];
-    else {
-      #pragma unroll
-      for(int j = 0; j < pack; ++j) word[i].v[j] = from_f32<real_t>(-INFINITY);
-    }
-  }
-  float edge_value = edge >= 0 ? to_f32(x[edge]) : -INFINITY;
-
-  // The teacher's distribution, meanwhile, and the student's logits at its
-  // tokens: all of them in the first CTA, for the loss, and a CTA's own, for the
-  // gradient. They are read before the barrier below, the gradient is written
-  // behind it: it may take the logits' place. A NaN stays one.
-  auto own = [&](int j) {
-    if(j < head || j >= vocabulary - tail) return 0 == rank;
-    int w = (j - head) / pack;
-    return w >= begin && w < end;
+  auto weight_of = [](float value) {
+    return value == -INFINITY ? 0.0f :
+      isnan(value) || value == INFINITY ? NAN : 1.0f;
   };
+
   float weight = weights ? weights[row] : 1.0f;
   peak_sum_t t { -INFINITY, 0.0f };
   for(int k = tid; k < entries; k += nt) {
     int64_t j = teacher.token(row * entries + k);
     bool used = j >= 0 && j < vocabulary && weight != 0;
-    float logit = used ? teacher.logit(row * entries + k) : -INFINITY;
     at[k] = used ? (int)j : -1;
-    p[k] = logit;
-    student[k] = used && (!rank || own((int)j)) ? to_f32(x[j]) : 0.0f;
-    t = merge(t, peak_sum_t { logit, logit == -INFINITY ? 0.0f :
-      isnan(logit) ? logit : 1.0f }, c);
+    p[k] = used ? teacher.logit(row * entries + k) : -INFINITY;
+    student[k] = used ? to_f32(x[j]) : 0.0f;
+    t = merge(t, peak_sum_t { p[k], weight_of(p[k]) }, c);
+  }
+  peak_sum_t s { -INFINITY, 0.0f };
+  #pragma unroll 4
+  for(int v = tid; v < vocabulary; v += nt) {
+    float value = to_f32(x[v]);
+    s = merge(s, peak_sum_t { value, weight_of(value) }, c);
   }
   t = warp_merge(t, c);
-  if(!lane) teacher_part[warp] = t;
-
-  // One pass over the student's logits.
-  float peak = edge_value;
-  #pragma unroll
-  for(int i = 0; i < held; ++i)
-    #pragma unroll
-    for(int j = 0; j < pack; ++j) peak = fmaxf(peak, to_f32(word[i].v[j]));
-  float base = peak == -INFINITY ? 0.0f : peak, sum = 0;
-  #pragma unroll
-  for(int i = 0; i < held; ++i)
-    #pragma unroll
-    for(int j = 0; j < pack; ++j)
-      sum += exp2_fast((to_f32(word[i].v[j]) - base) * c);
-  sum += exp2_fast((edge_value - base) * c);
-  peak_sum_t s { peak, sum };
-  for(int w = begin + held * nt + tid; w < end; w += nt) {
-    word_t more = x_words[w];
-    peak = s.peak;
-    #pragma unroll
-    for(int j = 0; j < pack; ++j) peak = fmaxf(peak, to_f32(more.v[j]));
-    base = peak == -INFINITY ? 0.0f : peak;
-    sum = s.sum * exp2_fast((s.peak - base) * c);
-    #pragma unroll
-    for(int j = 0; j < pack; ++j)
-      sum += exp2_fast((to_f32(more.v[j]) - base) * c);
-    s = peak_sum_t { peak, sum };
-  }
   s = warp_merge(s, c);
-  if(1 == ctas) {
-    if(!lane) part[warp] = s;
-    __syncthreads();
-  } else {
-    ptx::cluster_wait();                     // every CTA has started
-    if(lane < ctas)
-      cluster.map_shared_rank(part, lane)[rank * warps + warp] = s;
-    cluster.sync();
+  if(!lane) {
+    teacher_part[warp] = t;
+    part[warp] = s;
   }
-  s = peak_sum_t { -INFINITY, 0.0f };
-  #pragma unroll
-  for(int i = 0; i < parts / 32; ++i) {
-    int q = i * 32 + lane;
-    if(q < ctas * warps) s = merge(s, part[q], c);
-  }
-  s = warp_merge(s, c);
-  t = warp_merge(lane < warps ? teacher_part[lane] :
-    peak_sum_t { -INFINITY, 0.0f }, c);
+  __syncthreads();
+  const peak_sum_t nothing { -INFINITY, 0.0f };
+  t = warp_merge(lane < warps ? teacher_part[lane] : nothing, c);
+  s = warp_merge(lane < warps ? part[lane] : nothing, c);
   bool taught = t.peak > -INFINITY || isnan(t.sum);
   bool none = !taught || (s.peak == -INFINITY && !isnan(s.sum));
-
-  // From logits to probabilities, and the first CTA adds up the loss.
   float log_sum = logf(t.sum), log_mass = logf(s.sum), loss = 0;
   for(int k = tid; k < entries; k += nt) {
     float log_p = (p[k] - t.peak) / temperature - log_sum;
-    float prob = at[k] < 0 ? 0.0f : expf(log_p);
-    if(!rank && prob != 0 && !none) {
-      float log_q = (student[k] - s.peak) / temperature - log_mass;
-      loss += prob * (log_p - log_q);
-    }
+    float prob = taught && p[k] != -INFINITY ? expf(log_p) : 0.0f;
+    if(prob != 0)
+      loss += prob * (log_p - ((student[k] - s.peak) / temperature - log_mass));
+    else
+      at[k] = -1;
     p[k] = prob;
   }
-  if(!rank) {
-    #pragma unroll
-    for(int offset = 16; offset; offset /= 2)
-      loss += __shfl_xor_sync(0xffffffffu, loss, offset);
-    if(!lane) loss_part[warp] = loss;
-    __syncthreads();
-    if(!tid) {
-      loss = 0;
-      for(int w = 0; w < warps; ++w) loss += loss_part[w];
-      losses[row] = none ? 0.0f : temperature * temperature * loss;
-    }
+  #pragma unroll
+  for(int offset = 16; offset; offset /= 2)
+    loss += __shfl_xor_sync(0xffffffffu, loss, offset);
+  if(!lane) loss_part[warp] = loss;
+
+  float factor = none ? 0.0f : weight * temperature / s.sum;
+  #pragma unroll 4
+  for(int v = tid; v < vocabulary; v += nt)
+    g[v] = from_f32<real_t>(none ? 0.0f :
+      factor * exp2_fast((to_f32(x[v]) - s.peak) * c));
+  __syncthreads();
+  if(!tid) {
+    loss = 0;
+    for(int w = 0; w < warps; ++w) loss += loss_part[w];
+    losses[row] = none ? 0.0f : temperature * temperature * loss;
   }
-  if(want_grad) {
-    float factor = weight * temperature / s.sum;
-    auto slope = [&](float value) {
-      return none ? 0.0f : factor * exp2_fast((value - s.peak) * c);
-    };
-    word_t* g_words = (word_t*)(g + head);
-    #pragma unroll
-    for(int i = 0; i < held; ++i) {
-      int w = begin + i * nt + tid;
-      if(w < end) {
-        #pragma unroll
-        for(int j = 0; j < pack; ++j)
-          word[i].v[j] = from_f32<real_t>(slope(to_f32(word[i].v[j])));
-        store_streaming(g_words + w, word[i]);
-      }
-    }
-    for(int w = begin + held * nt + tid; w < end; w += nt) {
-      word_t more = x_words[w];
-      #pragma unroll
-      for(int j = 0; j < pack; ++j)
-        more.v[j] = from_f32<real_t>(slope(to_f32(more.v[j])));
-      store_streaming(g_words + w, more);
-    }
-    if(edge >= 0) g[edge] = from_f32<real_t>(slope(edge_value));
-    __syncthreads();
-    // The teacher's tokens in this CTA's part again, each with all of its
-    // entries.
-    for(int k = tid; k < entries && !none; k += nt) {
-      if(at[k] < 0 || !own(at[k])) continue;
-      float taken = 0;
-      for(int i = 0; i < entries; ++i)
-        if(at[i] == at[k]) taken += p[i];
-      g[at[k]] = from_f32<real_t>(slope(student[k]) -
-        weight * temperature * taken);
-    }
+  // The teacher's tokens again, each with all of its entries.
+  for(int k = tid; k < entries && !none; k += nt) {
+    if(at[k] < 0) continue;
+    float taken = 0;
+    for(int i = 0; i < entries; ++i)
+      if(at[i] == at[k]) taken += p[i];
+    g[at[k]] = from_f32<real_t>(factor *
+      exp2_fast((student[k] - s.peak) * c) - weight * temperature * taken);
   }
 }
 
@@ -281,11 +184,11 @@ distill_k(const real_t* logits, int64_t stride, int vocabulary, int ctas,
 // of them, the list of tokens in its part with their probabilities and the
 // student's logits, and of p and p (s - the greatest of these logits) the sums,
 // which is all that the loss needs: log q_j = (s_j - peak) / T - log mass.
-enum { distill_words = 4 };        // a thread's words in a landing buffer
+// A row of many words has a CTA of 512 threads, one to an SM; rows of less are
+// worked on by four CTAs of 128, whose barriers hide behind one another.
+enum { distill_words = 4,          // a thread's words in a landing buffer
+  distill_nt_large = 512, distill_nt_small = 128, distill_small_per_sm = 4 };
 
-#ifndef DOCC
-#define DOCC 4
-#endif
 struct distill_list_t {
   int listed, taught;
   float weight, entropy;           // entropy: sum of p log p over all entries
@@ -374,7 +277,8 @@ MGPU_DEVICE __forceinline__ float words_peak(
 }
 
 template<int nt, int pack, bool want_grad, typename real_t>
-__global__ void __launch_bounds__(nt + 64, nt == 512 ? 1 : DOCC)
+__global__ void __launch_bounds__(nt + 64, nt == distill_nt_large ? 1 :
+  distill_small_per_sm)
 distill_stream_k(const real_t* logits, int64_t stride, int count,
   int vocabulary, int log_ctas, int stages, distill_teacher_t teacher,
   float temperature, const float* weights, float* losses, real_t* grad,
@@ -616,7 +520,8 @@ distill_stream_k(const real_t* logits, int64_t stride, int count,
       }
       const uint64_t minus_base = ptx::make_pair(-base, -base);
       #pragma unroll
-      for(int i = 0; i < held; ++i)
+      for(int i = 0; i < held; ++i) {
+        if(w + i * nt >= end) break;         // the same for the whole CTA
         #pragma unroll
         for(int j = 0; j < pack; j += 2) {
           float2 power = ptx::pair_values(ptx::mul_pair(ptx::add_pair(
@@ -624,6 +529,7 @@ distill_stream_k(const real_t* logits, int64_t stride, int count,
           sums = ptx::add_pair(sums, ptx::make_pair(exp2_fast(power.x),
             exp2_fast(power.y)));
         }
+      }
     }
     peak_sum_t s { peak, ptx::pair_values(sums).x + ptx::pair_values(sums).y };
     s = merge(s, peak_sum_t { edge_value, edge_value == -INFINITY ? 0.0f :
@@ -695,6 +601,7 @@ distill_stream_k(const real_t* logits, int64_t stride, int count,
         take(word, end - w);
         #pragma unroll
         for(int i = 0; i < held; ++i) {
+          if(w + i * nt >= end) break;
           #pragma unroll
           for(int j = 0; j < pack; j += 2) {
             float2 power = ptx::pair_values(ptx::mul_pair(ptx::add_pair(
@@ -724,6 +631,26 @@ distill_stream_k(const real_t* logits, int64_t stride, int count,
   }
 }
 
+// How many clusters of `ctas` CTAs the device holds at a time; asked once for
+// each kernel, device, size of the cluster and number of stages.
+template<typename... tag_t, typename kernel_t>
+int resident_clusters(kernel_t kernel, cudaLaunchConfig_t config, int ctas,
+  int stages) {
+  static std::atomic<int> known[64][4][8];
+  int device = 0;
+  throw_on_error(cudaGetDevice(&device));
+  int log = ctas < 2 ? 0 : ctas < 4 ? 1 : ctas < 8 ? 2 : 3;
+  std::atomic<int>* at = device < 64 ? &known[device][log][stages & 7] : nullptr;
+  int clusters = at ? at->load(std::memory_order_relaxed) : 0;
+  if(!clusters) {
+    config.gridDim = dim3((unsigned)ctas);
+    throw_on_error(cudaOccupancyMaxActiveClusters(&clusters, kernel, &config));
+    if(clusters < 1) clusters = 1;
+    if(at) at->store(clusters, std::memory_order_relaxed);
+  }
+  return clusters;
+}
+
 template<bool want_grad, typename real_t, typename teacher_t, typename token_t>
 void distill_enqueue(const real_t* logits, int64_t stride, int count,
   int vocabulary, const token_t* tokens, const teacher_t* teacher, int entries,
@@ -746,28 +673,19 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  if(apart) {
-    enum { nt = 256 };
-    int ctas = 1;
-    while(ctas < distill_max_cluster && (int64_t)count * ctas < 296 &&
-      vocabulary / ctas > 4096) ctas *= 2;
-    config.gridDim = dim3((unsigned)((int64_t)count * ctas));
-    config.blockDim = dim3(nt);
-    config.dynamicSmemBytes = 12 * (size_t)entries;
-    attribute.val.clusterDim.x = (unsigned)ctas;
-    throw_on_error(cudaLaunchKernelEx(&config,
-      distill_k<nt, 1, want_grad, real_t>, logits, stride, vocabulary, ctas,
-      source, temperature, weights, losses, grad, grad_stride));
-    return;
+  if constexpr (want_grad) {
+    if(apart) {
+      enum { nt = 512 };
+      distill_apart_k<nt><<<(unsigned)count, nt, 12 * (size_t)entries,
+        stream>>>(logits, stride, vocabulary, source, temperature, weights,
+          losses, grad, grad_stride);
+      throw_on_error(cudaGetLastError());
+      return;
+    }
   }
-#ifndef DSMALL
-#define DSMALL (96 << 10)
-#endif
-#ifndef DC
-#define DC 0
-#endif
   auto launch = [&](auto threads) {
-    enum { nt = decltype(threads)::value, per_sm = nt == 512 ? 1 : DOCC,
+    enum { nt = decltype(threads)::value,
+      per_sm = nt == distill_nt_large ? 1 : distill_small_per_sm,
       stage_bytes = nt * distill_words * 16 };
     auto kernel = distill_stream_k<nt, 16 / (int)size, want_grad, real_t>;
     // What an SM has, less the shared variables of fixed size.
@@ -777,23 +695,40 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
     stages = stages < 3 ? 3 : stages > 6 ? 6 : stages;
     set_dynamic_smem<decltype(threads), std::integral_constant<bool, want_grad>,
       real_t>(kernel, 224 << 10);
-    // Clusters where there are too few rows for all SMs, or for whole rounds of
-    // them.
-    int slots = 148 * per_sm, ctas = 1;
-    while(ctas < distill_max_cluster && row_bytes / ctas > 2 * stage_bytes &&
-      (int64_t)count * ctas < 6 * slots) ctas *= 2;
-    if(DC) ctas = DC;
-    int log_ctas = ctas < 2 ? 0 : ctas < 4 ? 1 : ctas < 8 ? 2 : 3;
-    attribute.val.clusterDim.x = (unsigned)ctas;
     config.blockDim = dim3(nt + 64);
     config.dynamicSmemBytes = (size_t)stages * stage_bytes + lists;
-    config.gridDim = dim3((unsigned)(min(count, slots / ctas) * ctas));
+    // CTAs to a row: rounds of rows times what each takes, a round's barriers
+    // being worth about 32 KB.
+    int ctas = 1, clusters = 1;
+    int64_t least = 0;
+    for(int n = 1; n <= distill_max_cluster; n *= 2) {
+      if(n > 1 && row_bytes / n < stage_bytes) break;
+      attribute.val.clusterDim.x = (unsigned)n;
+      int most = resident_clusters<decltype(threads), std::integral_constant<
+        bool, want_grad>, real_t>(kernel, config, n, stages);
+      int64_t cost = div_up((int64_t)count, (int64_t)most) *
+        (row_bytes / n + (32 << 10));
+      if(!least || cost < least) {
+        least = cost;
+        ctas = n;
+        clusters = most;
+      }
+    }
+    int log_ctas = ctas < 2 ? 0 : ctas < 4 ? 1 : ctas < 8 ? 2 : 3;
+    attribute.val.clusterDim.x = (unsigned)ctas;
+    config.gridDim = dim3((unsigned)(min(count, clusters) * ctas));
     throw_on_error(cudaLaunchKernelEx(&config, kernel, logits, stride, count,
       vocabulary, log_ctas, stages, source, temperature, weights, losses, grad,
       grad_stride, timeout_ns));
   };
-  if(row_bytes > DSMALL) launch(std::integral_constant<int, 512>());
-  else launch(std::integral_constant<int, 128>());
+  // Measured with 2,048 rows of 64 KB (loss): 30.5 us in small CTAs, 57.8 us in
+  // large ones; with gradient, 509 rows of 200 KB: 61 us small, 46 us large, and
+  // 4,096 rows of 256 KB: 565 us small (150 MB of rows under way push one another
+  // out of the L2), 426 us large.
+  if(row_bytes > (96 << 10))
+    launch(std::integral_constant<int, distill_nt_large>());
+  else
+    launch(std::integral_constant<int, distill_nt_small>());
 }
 
 } // namespace detail

@@ -320,6 +320,47 @@ def test_distill_strides_and_in_place(mgpu, dtype, extra, offset):
         assert (around[:, 1000:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", REALS)
+@pytest.mark.parametrize("vocab", [1, 7, 1000, 33001])
+def test_distill_gradient_aligned_apart_from_the_logits(mgpu, dtype, vocab):
+    g = gen(19)
+    x = (randn(g, 5, vocab) * 3).to(dtype)
+    at, teacher = teacher_of(g, 5, vocab, 40)
+    weights = torch.tensor([1.0, 0.5, 0.0, 2.0, 1.0], device="cuda")
+    x[4] = -float("inf")
+    check_distill(mgpu, strided(x, 3), at, teacher, weights,
+                  out=strided(x * 0, 3, 1))
+    check_distill(mgpu, strided(x, 1), at, teacher, weights,
+                  out=strided(x * 0, 2))
+
+
+@pytest.mark.parametrize("grad_rows", [1, 40, 700])
+@pytest.mark.parametrize("vocab", [5, 3000, 60000, 140001])
+def test_distill_numbers_of_rows(mgpu, grad_rows, vocab):
+    """Rows that stay with their CTAs for several rounds, in clusters of every
+    size; a sample of them is compared."""
+    g = gen(vocab)
+    logits = (randn(g, grad_rows, vocab) * 3).bfloat16()
+    at, teacher = teacher_of(g, grad_rows, vocab, 20)
+    loss, grad = mgpu.distill_loss_gradient(logits, at, teacher)
+    rows = sorted({0, grad_rows // 2, grad_rows - 1})
+    want, slope, loss_bound, grad_bound = (torch.from_numpy(v) for v in
+        ref.distill(logits[rows], at[rows], teacher[rows], None, 1.0))
+    close(loss[rows], want, loss_bound)
+    close(grad[rows], slope, grad_bound)
+    assert torch.equal(loss, mgpu.distill_loss(logits, at, teacher))
+    # Every row by itself: the loss from the gradient's own probabilities.
+    few = (at >= 0) & (at < vocab)
+    p = torch.softmax(torch.where(few, teacher, -float("inf")).double(), 1)
+    p = torch.nan_to_num(p)
+    log_q = torch.log_softmax(logits.double(), 1)
+    plain = torch.special.entr(p).sum(1).neg() - (
+        p * log_q.gather(1, at.clamp(0, vocab - 1))).sum(1)
+    # 32-bit sums of `vocab` weights, and of 20 products of order 30.
+    assert torch.allclose(loss.double(), plain, rtol=1e-4, atol=1e-4)
+    assert grad.float().sum(1).abs().max() <= 2.0 ** -8 * 2.01
+
+
 def test_distill_rows_without_a_distribution(mgpu):
     inf = float("inf")
     x = torch.randn(7, 300, device="cuda", generator=gen(14))
