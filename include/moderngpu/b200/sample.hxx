@@ -54,6 +54,12 @@ MGPU_DEVICE __forceinline__ float key_value(uint32_t key) {
 // tokens, the same one in every pass, so that after the first pass the row comes
 // from the L1 (or the L2, where it is too long for it).
 //
+// Few tokens kept by top-k: every CTA finds the step of a histogram of its own
+// part that holds its own top_k-th token and lists the tokens down to this step,
+// which hold the row's greatest top_k. The first CTA sorts the lists of all and
+// goes on alone.
+//
+// Otherwise:
 //   pass 1  the greatest logit
 //   pass 2  a histogram over the distance from it, in steps of T / 64: of counts
 //           for top-k; of weights in fixed point, relative to the step's own
@@ -63,38 +69,46 @@ MGPU_DEVICE __forceinline__ float key_value(uint32_t key) {
 //           few tokens above the border the list holds those too, and the first
 //           CTA goes on alone, on the list.
 //   pass 4  the weight that is left in each warp's run; the run that holds the
-//           drawn number is searched by its warp.
+//           drawn number is searched by its CTA.
 // Where the steps hold more tokens than the list takes, their range of logits
 // is halved with exact sums until it fits or is a single value, whose tokens
 // are then taken by index.
+//
+// What a warp finds it tells all CTAs at once, and every warp adds up what all
+// warps told: one barrier of the cluster (1,300 cycles) to an exchange, and none
+// of the CTA.
 
 enum { sample_bins = 2048, sample_steps = 64, sample_list = 1024,
-  sample_max_cluster = 8 };
+  sample_max_cluster = 8, sample_powers = 64, sample_groups = 64 };
 
-// What the CTAs of a cluster tell one another.
+// What a warp tells all CTAs of its cluster.
 struct sample_news_t {
-  double a, b, c;
+  double a, b;
   uint32_t p, q;
   int i, j;
 };
 
 template<int nt>
 struct sample_shared_t {
-  enum { warps = nt / 32 };
+  enum { warps = nt / 32, runs = sample_max_cluster * warps };
   uint32_t hist[sample_bins];
   unsigned long long list[sample_list];
-  sample_news_t news[2][sample_max_cluster];
-  double run_sums[sample_max_cluster * warps];
-  double warp_sums[2][warps];
-  double fold[warps];
-  int list_count;
-  int hit;
+  double list_weights[sample_list];
+  sample_news_t news[2][runs];
+  double powers[sample_powers];              // 2^(i / 64)
+  // Of 32 threads' steps each: weight and tokens.
+  double group_weights[sample_groups], group_tokens[sample_groups];
+  double band_before, band_tokens;
+  int band_lo, band_hi;
+  double fold[2][warps];
+  int list_count, hit;
 };
 
 template<int nt, typename real_t>
 struct sample_cta_t {
   enum { warps = nt / 32, pack = 16 / (int)sizeof(real_t),
-    each_list = sample_list / nt };
+    each_list = sample_list / nt, runs = sample_max_cluster * warps,
+    each_lane = runs / 32 };
   typedef pack_t<real_t, pack> word_t;
   typedef sample_shared_t<nt> shared_t;
   struct band_t { int lo, hi; double tokens, inside; };
@@ -110,7 +124,7 @@ struct sample_cta_t {
 
   float peak, inv_temperature;
   uint32_t peak_key;
-  double scale;
+  double log2_scale;   // log2(e) / T
   uint32_t least;      // what is kept: keys above this one,
   int last;            // and those equal to it up to this index
 
@@ -122,10 +136,14 @@ struct sample_cta_t {
     warp((int)threadIdx.x / 32), exchanges(0), least(0), last(vocabulary_) {
     run = rank * warps + warp;
     shift = (int)((uintptr_t)x % 16 / sizeof(real_t));
-    int64_t end = (int64_t)vocabulary + shift, step = 32 * pack;
-    int64_t length = div_up(div_up(end, (int64_t)ctas * warps), step) * step;
+    int64_t end = (int64_t)vocabulary + shift, length = run_length();
     run_begin = min(length * run, end);
     run_end = min(run_begin + length, end);
+  }
+  MGPU_DEVICE int64_t run_length() const {
+    int64_t step = 32 * pack;
+    return div_up(div_up((int64_t)vocabulary + shift, (int64_t)ctas * warps),
+      step) * step;
   }
 
   // f(logit, index) for the tokens of this warp's run.
@@ -167,74 +185,109 @@ struct sample_cta_t {
       f(to_f32(x[i - shift]), (int)(i - shift));
   }
 
-  template<typename type_t, typename op_t>
-  MGPU_DEVICE type_t fold(type_t v, op_t op) {
-    type_t* parts = (type_t*)shared.fold;
+  //////////////////////////////////////////////////////////////////////////////
+  // Sums.
+
+  MGPU_DEVICE static double warp_sum(double v) {
     #pragma unroll
     for(int offset = 16; offset; offset /= 2)
-      v = op(v, __shfl_xor_sync(0xffffffffu, v, offset));
-    if(!lane) parts[warp] = v;
-    __syncthreads();
-    v = parts[0];
+      v += __shfl_xor_sync(0xffffffffu, v, offset);
+    return v;
+  }
+  MGPU_DEVICE double upto(double v) const {
     #pragma unroll
-    for(int w = 1; w < warps; ++w) v = op(v, parts[w]);
+    for(int offset = 1; offset < 32; offset *= 2) {
+      double y = __shfl_up_sync(0xffffffffu, v, offset);
+      if(lane >= offset) v += y;
+    }
+    return v;
+  }
+  // Over the CTA's threads, in the order of the warps.
+  MGPU_DEVICE double cta_upto(double v) {
+    v = upto(v);
+    if(31 == lane) shared.fold[0][warp] = v;
+    __syncthreads();
+    double others = upto(lane < warps ? shared.fold[0][lane] : 0.0);
+    others = __shfl_sync(0xffffffffu, others, (warp + 31) % 32);
+    __syncthreads();
+    return warp ? v + others : v;
+  }
+  MGPU_DEVICE double cta_sum(double v) {
+    v = warp_sum(v);
+    if(!lane) shared.fold[0][warp] = v;
+    __syncthreads();
+    v = warp_sum(lane < warps ? shared.fold[0][lane] : 0.0);
     __syncthreads();
     return v;
   }
-  MGPU_DEVICE double fold_sum(double v) {
-    return fold(v, [](double a, double b) { return a + b; });
-  }
-  MGPU_DEVICE double fold_most(double v) {
-    return fold(v, [](double a, double b) { return a < b ? b : a; });
-  }
-  MGPU_DEVICE int fold_min(int v) {
-    return fold(v, [](int a, int b) { return a < b ? a : b; });
-  }
-  MGPU_DEVICE int fold_max(int v) {
-    return fold(v, [](int a, int b) { return a < b ? b : a; });
-  }
-  MGPU_DEVICE uint32_t fold_max(uint32_t v) {
-    return fold(v, [](uint32_t a, uint32_t b) { return a < b ? b : a; });
-  }
-
-  // Inclusive sums over the CTA's threads.
-  MGPU_DEVICE double2 scan(double a, double b) {
-    double2 sum = make_double2(a, b);
-    #pragma unroll
-    for(int offset = 1; offset < 32; offset *= 2) {
-      double y = __shfl_up_sync(0xffffffffu, sum.x, offset);
-      double z = __shfl_up_sync(0xffffffffu, sum.y, offset);
-      if(lane >= offset) { sum.x += y; sum.y += z; }
-    }
-    if(31 == lane) {
-      shared.warp_sums[0][warp] = sum.x;
-      shared.warp_sums[1][warp] = sum.y;
-    }
+  MGPU_DEVICE uint32_t cta_max(uint32_t v) {
+    uint32_t* parts = (uint32_t*)shared.fold[0];
+    v = __reduce_max_sync(0xffffffffu, v);
+    if(!lane) parts[warp] = v;
     __syncthreads();
-    for(int w = 0; w < warp; ++w) {
-      sum.x += shared.warp_sums[0][w];
-      sum.y += shared.warp_sums[1][w];
-    }
+    v = __reduce_max_sync(0xffffffffu, lane < warps ? parts[lane] : 0u);
     __syncthreads();
-    return sum;
+    return v;
   }
+  MGPU_DEVICE uint32_t cta_min(uint32_t v) { return ~cta_max(~v); }
 
-  // Every CTA's news (the same in all of its threads) to every CTA. Two sets
-  // of slots: one is written again only behind a barrier that its readers have
-  // passed.
+  // Every warp's news (the same in its lanes) to every CTA. Two sets of slots:
+  // one is written again only behind a barrier that its readers have passed.
   MGPU_DEVICE const sample_news_t* share(const sample_news_t& mine) {
+    if(!exchanges) ptx::cluster_wait();      // every CTA has started
     int set = exchanges++ & 1;
-    if(tid < ctas)
-      cluster.map_shared_rank(&shared, tid)->news[set][rank] = mine;
+    if(lane < ctas)
+      cluster.map_shared_rank(&shared, lane)->news[set][run] = mine;
     cluster.sync();
     return shared.news[set];
   }
+  // f(news) for a part of all warps' news in each lane.
+  template<typename func_t>
+  MGPU_DEVICE __forceinline__ void all_news(const sample_news_t* news,
+    func_t f) const {
+    #pragma unroll
+    for(int i = 0; i < each_lane; ++i) {
+      int r = i * 32 + lane;
+      if(r < ctas * warps) f(news[r]);
+    }
+  }
+
+  //////////////////////////////////////////////////////////////////////////////
+  // Weights.
 
   MGPU_DEVICE bool kept(uint32_t key, int v) const {
     return key > least || (key == least && v <= last);
   }
+  // 2^(i / 64), i < 64, in shared memory.
+  MGPU_DEVICE void make_powers() {
+    if(tid < sample_powers)
+      shared.powers[tid] = exp2((double)tid / sample_powers);
+  }
+  // exp((value - peak) / T) to about 1e-14 (the rounding of log2(e) / T times a
+  // distance of up to 60). With y = (value - peak) log2(e) / T = i / 64 + r, r
+  // at most 1/128 in size, it is 2^(i / 64) 2^r: a power from the table and the
+  // Taylor series of exp(r ln 2), whose sixth-degree term is below 4e-17. Eleven
+  // operations of 64 bits; the library's exp takes several times as many, and
+  // these passes are bound by them. Below 2^-1000 it is 0.
   MGPU_DEVICE double weight(float value) const {
-    return value == peak ? 1.0 : exp(((double)value - (double)peak) * scale);
+    if(value == peak) return 1.0;
+    const double magic = 1.5 * 70368744177664.0;       // 1.5 * 2^46: ulp 2^-6
+    double d = (double)value - (double)peak;
+    double z = fma(d, log2_scale, magic);
+    double r = fma(d, log2_scale, -(z - magic));
+    int i = __double2loint(z);
+    // ln2^n / n!
+    double p = 1.3333558146428443e-3;
+    p = fma(p, r, 9.618129107628477e-3);
+    p = fma(p, r, 5.550410866482158e-2);
+    p = fma(p, r, 2.402265069591007e-1);
+    p = fma(p, r, 6.931471805599453e-1);
+    double t = shared.powers[i & (sample_powers - 1)];
+    t = fma(t, p * r, t);
+    int exponent = i >> 6;
+    double w = __hiloint2double(__double2hiint(t) + exponent * (1 << 20),
+      __double2loint(t));
+    return d * log2_scale < -1000.0 ? 0.0 : w;
   }
   template<bool by_count>
   MGPU_DEVICE double size(float value) const {
@@ -248,62 +301,58 @@ struct sample_cta_t {
     return (int)fminf(distance * (float)sample_steps, sample_bins - 1.0f);
   }
 
-  MGPU_DEVICE uint32_t find_peak() {
+  // A NaN has the greatest key of all.
+  MGPU_DEVICE uint32_t part_peak() const {
     uint32_t key = 0;
     each([&](float value, int) {
       key = max(key, isnan(value) ? 0xffffffffu : order_key(value));
     });
-    sample_news_t mine = { };
-    mine.p = fold_max(key);
-    ptx::cluster_wait();                     // every CTA has started
-    const sample_news_t* news = share(mine);
-    key = 0;
-    for(int r = 0; r < ctas; ++r) key = max(key, news[r].p);
-    return key;
+    return __reduce_max_sync(0xffffffffu, key);
   }
-
+  MGPU_DEVICE void find_peak() {
+    sample_news_t mine = { };
+    mine.p = part_peak();
+    const sample_news_t* news = share(mine);
+    uint32_t key = 0;
+    all_news(news, [&](const sample_news_t& n) { key = max(key, n.p); });
+    peak_key = __reduce_max_sync(0xffffffffu, key);
+  }
   MGPU_DEVICE int first_of(uint32_t wanted) {
-    int at = vocabulary;
+    uint32_t at = 0xffffffffu;
     each([&](float value, int v) {
-      if(order_key(value) == wanted && v < at) at = v;
+      if(order_key(value) == wanted) at = min(at, (uint32_t)v);
     });
     sample_news_t mine = { };
-    mine.i = fold_min(at);
+    mine.p = __reduce_min_sync(0xffffffffu, at);
     const sample_news_t* news = share(mine);
-    at = vocabulary;
-    for(int r = 0; r < ctas; ++r) at = min(at, news[r].i);
-    return at;
+    at = 0xffffffffu;
+    all_news(news, [&](const sample_news_t& n) { at = min(at, n.p); });
+    return (int)__reduce_min_sync(0xffffffffu, at);
   }
 
   //////////////////////////////////////////////////////////////////////////////
-  // Sums of the runs, in the order of the vocabulary.
+  // Sums of the runs, in the order of the vocabulary: the `a` of the news.
 
-  // Each warp's number (the same in its lanes) to every CTA.
-  MGPU_DEVICE void share_run_sum(double mine) {
-    if(lane < ctas)
-      cluster.map_shared_rank(&shared, lane)->run_sums[run] = mine;
-    cluster.sync();
+  // All runs together, in every lane.
+  MGPU_DEVICE double total_of_runs(const sample_news_t* news) const {
+    double sum = 0;
+    all_news(news, [&](const sample_news_t& n) { sum += n.a; });
+    return warp_sum(sum);
   }
   // The first run with a sum for which test(sum up to its end), and the sum
   // before it; where there is none, the last run with a sum; -1 where all are
   // 0. The same in every thread of the cluster.
   template<typename test_t>
-  MGPU_DEVICE int find_run(test_t test, double& before) {
-    enum { each_lane = sample_max_cluster * warps / 32 };
+  MGPU_DEVICE int find_run(const sample_news_t* news, test_t test,
+    double& before) const {
     double own[each_lane], sum = 0;
     #pragma unroll
     for(int i = 0; i < each_lane; ++i) {
       int r = lane * each_lane + i;
-      own[i] = r < ctas * warps ? shared.run_sums[r] : 0.0;
+      own[i] = r < ctas * warps ? news[r].a : 0.0;
       sum += own[i];
     }
-    double ahead = sum;
-    #pragma unroll
-    for(int offset = 1; offset < 32; offset *= 2) {
-      double y = __shfl_up_sync(0xffffffffu, ahead, offset);
-      if(lane >= offset) ahead += y;
-    }
-    ahead = __shfl_up_sync(0xffffffffu, ahead, 1);
+    double ahead = __shfl_up_sync(0xffffffffu, upto(sum), 1);
     if(!lane) ahead = 0;
     int found = -1, any = -1;
     double found_before = 0, any_before = 0;
@@ -331,20 +380,6 @@ struct sample_cta_t {
     before = __shfl_sync(0xffffffffu, any_before, from);
     return __shfl_sync(0xffffffffu, any, from);
   }
-  // All runs together, in every thread.
-  MGPU_DEVICE double total_of_runs() const {
-    enum { each_lane = sample_max_cluster * warps / 32 };
-    double sum = 0;
-    #pragma unroll
-    for(int i = 0; i < each_lane; ++i) {
-      int r = lane * each_lane + i;
-      sum += r < ctas * warps ? shared.run_sums[r] : 0.0;
-    }
-    #pragma unroll
-    for(int offset = 16; offset; offset /= 2)
-      sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    return sum;
-  }
   // The CTA whose run `found` is searches it: size(value, index) of the tokens
   // is added up in order, from `before`, and the first token with a size whose
   // sum passes test is the result, else the last one with a size. Each warp adds
@@ -352,9 +387,7 @@ struct sample_cta_t {
   template<typename size_t_, typename test_t>
   MGPU_DEVICE int search_run(int found, double before, size_t_ size,
     test_t test) {
-    int64_t length = div_up(div_up((int64_t)vocabulary + shift,
-      (int64_t)ctas * warps), (int64_t)(32 * pack)) * (32 * pack);
-    int64_t begin = length * found;
+    int64_t length = run_length(), begin = length * found;
     int64_t end = min(begin + length, (int64_t)vocabulary + shift);
     int64_t part = div_up(div_up(length, (int64_t)warps), (int64_t)32) * 32;
     int64_t part_begin = min(begin + part * warp, end);
@@ -362,16 +395,14 @@ struct sample_cta_t {
     double sum = 0;
     for(int64_t a = part_begin + lane; a < part_end; a += 32)
       if(a >= shift) sum += size(to_f32(x[a - shift]), (int)(a - shift));
-    #pragma unroll
-    for(int offset = 16; offset; offset /= 2)
-      sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    if(!lane) shared.warp_sums[0][warp] = sum;
+    sum = warp_sum(sum);
+    if(!lane) shared.fold[0][warp] = sum;
     if(!tid) shared.hit = -1;
     __syncthreads();
     int chosen = -1;
     double chosen_before = 0;
     for(int w = 0; w < warps; ++w) {
-      double own = shared.warp_sums[0][w];
+      double own = shared.fold[0][w];
       if(own > 0) {
         chosen = w;
         chosen_before = before;
@@ -387,21 +418,15 @@ struct sample_cta_t {
         int64_t a = first + lane;
         double own = a >= shift && a < part_end ?
           size(to_f32(x[a - shift]), (int)(a - shift)) : 0.0;
-        double upto = own;
-        #pragma unroll
-        for(int offset = 1; offset < 32; offset *= 2) {
-          double y = __shfl_up_sync(0xffffffffu, upto, offset);
-          if(lane >= offset) upto += y;
-        }
+        double sum = upto(own);
         unsigned some = __ballot_sync(0xffffffffu, own > 0);
-        unsigned hits = __ballot_sync(0xffffffffu,
-          own > 0 && test(before + upto));
+        unsigned hits = __ballot_sync(0xffffffffu, own > 0 && test(before + sum));
         if(hits) {
           at = (int)(first - shift) + __ffs(hits) - 1;
           done = true;
         } else if(some)
           at = (int)(first - shift) + 31 - __clz(some);
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        before += __shfl_sync(0xffffffffu, sum, 31);
       }
       if(!lane) shared.hit = at;
     }
@@ -414,20 +439,22 @@ struct sample_cta_t {
     auto one = [&](float value, int v) {
       return order_key(value) == wanted && kept(wanted, v) ? 1.0 : 0.0;
     };
-    int mine = 0;
-    each([&](float value, int v) { mine += one(value, v) > 0; });
-    share_run_sum((double)__reduce_add_sync(0xffffffffu, mine));
+    int count = 0;
+    each([&](float value, int v) { count += one(value, v) > 0; });
+    sample_news_t mine = { };
+    mine.a = (double)__reduce_add_sync(0xffffffffu, count);
+    const sample_news_t* news = share(mine);
     auto test = [&](double sum) { return sum >= nth; };
     double before = 0;
-    int found = find_run(test, before);
+    int found = find_run(news, test, before);
     sample_news_t told = { };
     told.i = -1;
     if(found >= 0 && found / warps == rank)
       told.i = search_run(found, before, one, test);
-    const sample_news_t* news = share(told);
+    news = share(told);
     int at = -1;
-    for(int r = 0; r < ctas; ++r) at = max(at, news[r].i);
-    return at;
+    all_news(news, [&](const sample_news_t& n) { at = max(at, n.i); });
+    return __reduce_max_sync(0xffffffffu, at);
   }
 
   //////////////////////////////////////////////////////////////////////////////
@@ -436,12 +463,16 @@ struct sample_cta_t {
   // The border is where the running count reaches `target`, or the running
   // weight `target` times the weight of all.
 
+  MGPU_DEVICE void clear_hist() {
+    for(int b = tid; b < sample_bins; b += nt) shared.hist[b] = 0;
+    __syncthreads();
+  }
+
   template<bool by_count>
   MGPU_DEVICE band_t find_band(double target) {
     // Fixed-point weights: a step's sum stays below 2^32 whatever it holds.
     float unit = by_count ? 1.0f : fminf(4096.0f, 2147483648.0f / vocabulary);
-    for(int b = tid; b < sample_bins; b += nt) shared.hist[b] = 0;
-    __syncthreads();
+    clear_hist();
     each([&](float value, int v) {
       if(!kept(order_key(value), v)) return;
       float d = distance(value);
@@ -455,23 +486,33 @@ struct sample_cta_t {
       }
       atomicAdd(&shared.hist[b], add);
     });
+    if(!tid) {
+      shared.band_lo = shared.band_hi = sample_bins;
+      shared.band_before = shared.band_tokens = 0;
+    }
     cluster.sync();
 
-    // Each CTA adds up a slice of the steps, a few of them to a thread.
+    // Each CTA adds up a slice of the steps, a few neighbouring ones to a
+    // thread; a warp's are a group.
     enum { most = sample_bins / nt };
     int slice = sample_bins / ctas, each_thread = div_up(slice, (int)nt);
+    int active = slice / (32 * each_thread);   // warps with steps
     int first = rank * slice + tid * each_thread;
-    int mine_count = tid * each_thread < slice ? each_thread : 0;
     double weights[most], tokens[most], weight_sum = 0, token_sum = 0;
     // A token adds at least this much.
     double fewest = by_count ? 1.0 : (double)unit * 0.984 - 0.5;
     #pragma unroll
     for(int i = 0; i < most; ++i) {
       weights[i] = tokens[i] = 0;
-      if(i < mine_count) {
+      if(warp < active && i < each_thread) {
+        uint32_t parts[sample_max_cluster];
+        #pragma unroll
+        for(int r = 0; r < sample_max_cluster; ++r)
+          parts[r] = r < ctas ?
+            cluster.map_shared_rank(&shared, r)->hist[first + i] : 0;
         double sum = 0;
-        for(int r = 0; r < ctas; ++r)
-          sum += cluster.map_shared_rank(&shared, r)->hist[first + i];
+        #pragma unroll
+        for(int r = 0; r < sample_max_cluster; ++r) sum += parts[r];
         weights[i] = by_count ? sum :
           sum * exp(-(double)(first + i) / sample_steps);
         tokens[i] = fewest > 0 ? sum / fewest : sum * 1e30;
@@ -479,55 +520,67 @@ struct sample_cta_t {
       weight_sum += weights[i];
       token_sum += tokens[i];
     }
-    double2 sums = scan(weight_sum, token_sum);
-    sample_news_t mine = { };
-    mine.a = fold_most(sums.x);
-    mine.b = fold_most(sums.y);
-    const sample_news_t* news = share(mine);
-    double total = 0, all_tokens = 0, at = 0, at_tokens = 0;
-    for(int r = 0; r < ctas; ++r) {
-      if(r == rank) {
-        at = total + sums.x - weight_sum;
-        at_tokens = all_tokens + sums.y - token_sum;
+    double at = upto(weight_sum), at_tokens = upto(token_sum);
+    int group = rank * active + warp;
+    if(warp < active) {
+      double w = __shfl_sync(0xffffffffu, at, 31);
+      double t = __shfl_sync(0xffffffffu, at_tokens, 31);
+      if(lane < ctas) {
+        shared_t* there = cluster.map_shared_rank(&shared, lane);
+        there->group_weights[group] = w;
+        there->group_tokens[group] = t;
       }
-      total += news[r].a;
-      all_tokens += news[r].b;
     }
+    cluster.sync();
+    // Two groups to a lane: what is in front of this warp's, and of all.
+    int groups = ctas * active;
+    double w0 = 2 * lane < groups ? shared.group_weights[2 * lane] : 0.0;
+    double w1 = 2 * lane + 1 < groups ? shared.group_weights[2 * lane + 1] : 0.0;
+    double t0 = 2 * lane < groups ? shared.group_tokens[2 * lane] : 0.0;
+    double t1 = 2 * lane + 1 < groups ? shared.group_tokens[2 * lane + 1] : 0.0;
+    double w_upto = upto(w0 + w1), t_upto = upto(t0 + t1);
+    double total = __shfl_sync(0xffffffffu, w_upto, 31);
+    double all_tokens = __shfl_sync(0xffffffffu, t_upto, 31);
+    double w_front = w_upto - (group & 1 ? w1 : w0 + w1);
+    double t_front = t_upto - (group & 1 ? t1 : t0 + t1);
+    at += __shfl_sync(0xffffffffu, w_front, group / 2 % 32) - weight_sum;
+    at_tokens += __shfl_sync(0xffffffffu, t_front, group / 2 % 32) - token_sum;
     // Sum and total are each off by at most 0.51 / unit + 1e-5 of the total.
     double slack = by_count ? 0.0 : (2.0 / unit + 5e-5) * total;
     double goal = by_count ? target : target * total;
-    int lo = sample_bins, hi = sample_bins;
-    double lo_tokens = 0, hi_tokens = 0;
+    // The thread whose steps pass a border tells all CTAs, unless the sum was
+    // past it before.
     #pragma unroll
     for(int i = 0; i < most; ++i) {
-      if(i < mine_count) {
-        at += weights[i];
-        if(lo == sample_bins && at >= goal - slack) {
-          lo = first + i;
-          lo_tokens = at_tokens;
-        }
+      if(warp < active && i < each_thread) {
+        double to = at + weights[i];
+        bool is_lo = to >= goal - slack && (at < goal - slack ||
+          0 == first + i);
+        bool is_hi = to >= goal + slack && (at < goal + slack ||
+          0 == first + i);
+        if(is_lo || is_hi)
+          for(int r = 0; r < ctas; ++r) {
+            shared_t* there = cluster.map_shared_rank(&shared, r);
+            if(is_lo) {
+              there->band_lo = first + i;
+              there->band_before = at_tokens;
+            }
+            if(is_hi) {
+              there->band_hi = first + i;
+              there->band_tokens = at_tokens + tokens[i];
+            }
+          }
+        at = to;
         at_tokens += tokens[i];
-        if(hi == sample_bins && at >= goal + slack) {
-          hi = first + i;
-          hi_tokens = at_tokens;
-        }
       }
     }
-    mine.i = fold_min(lo);
-    mine.j = fold_min(hi);
-    mine.a = fold_most(lo == mine.i ? lo_tokens : 0.0);
-    mine.b = fold_most(hi == mine.j ? hi_tokens : 0.0);
-    news = share(mine);
-    band_t band { sample_bins, sample_bins, all_tokens, 0 };
-    double before = 0;
-    for(int r = ctas - 1; r >= 0; --r) {
-      if(news[r].i < sample_bins) { band.lo = news[r].i; before = news[r].a; }
-      if(news[r].j < sample_bins) {
-        band.hi = news[r].j;
-        band.tokens = news[r].b;
-      }
+    cluster.sync();
+    band_t band { shared.band_lo, shared.band_hi, shared.band_tokens, 0 };
+    double before = shared.band_before;
+    if(band.hi == sample_bins) {
+      band.hi = sample_bins - 1;
+      band.tokens = all_tokens;
     }
-    band.hi = min(band.hi, sample_bins - 1);
     if(band.lo > band.hi) {
       band.lo = 0;
       before = 0;
@@ -539,11 +592,13 @@ struct sample_cta_t {
   //////////////////////////////////////////////////////////////////////////////
   // The list, in the first CTA.
 
+  MGPU_DEVICE static unsigned long long entry(uint32_t key, int v) {
+    return (unsigned long long)key << 32 | (0xffffffffu - v);
+  }
   MGPU_DEVICE void append(uint32_t key, int v) {
     shared_t* first = cluster.map_shared_rank(&shared, 0);
     int at = atomicAdd(&first->list_count, 1);
-    if(at < sample_list)
-      first->list[at] = (unsigned long long)key << 32 | (0xffffffffu - v);
+    if(at < sample_list) first->list[at] = entry(key, v);
   }
   MGPU_DEVICE uint32_t list_key(int i) const {
     return (uint32_t)(shared.list[i] >> 32);
@@ -551,9 +606,10 @@ struct sample_cta_t {
   MGPU_DEVICE int list_index(int i) const {
     return (int)(0xffffffffu - (uint32_t)shared.list[i]);
   }
-  // The greatest first; equal keys by index.
+  // The greatest first; equal keys by index. A bitonic network: what stays
+  // within 64 entries is a warp's own.
   MGPU_DEVICE void sort_list(int count) {
-    int n = 2;
+    int n = 64;
     while(n < count) n *= 2;
     for(int i = count + tid; i < n; i += nt) shared.list[i] = 0;
     __syncthreads();
@@ -567,11 +623,13 @@ struct sample_cta_t {
             shared.list[i + j] = a;
           }
         }
-        __syncthreads();
+        if(j > 32 || (1 == j && k >= 64)) __syncthreads();
+        else __syncwarp();
       }
+    __syncthreads();
   }
   // The first place, in the list's order, of an entry with a size for which
-  // test(the sum up to it); else the last entry with a size. `sum`: of all.
+  // test(the sum up to it); else the last entry with a size.
   template<typename size_t_, typename test_t>
   MGPU_DEVICE int search_list(int count, size_t_ size, test_t test) {
     double own[each_list], sum = 0;
@@ -581,63 +639,211 @@ struct sample_cta_t {
       own[i] = e < count ? size(e) : 0.0;
       sum += own[i];
     }
-    double at = scan(sum, 0).x - sum;
-    int found = sample_list, any = -1;
+    double at = cta_upto(sum) - sum;
+    uint32_t found = 0xffffffffu, any = 0;
     #pragma unroll
     for(int i = 0; i < each_list; ++i) {
       at += own[i];
       if(own[i] > 0) {
-        any = tid * each_list + i;
-        if(found == sample_list && test(at)) found = any;
+        any = tid * each_list + i + 1;
+        if(0xffffffffu == found && test(at)) found = any - 1;
       }
     }
-    found = fold_min(found);
-    any = fold_max(any);
-    return found < sample_list ? found : any;
-  }
-  template<typename size_t_>
-  MGPU_DEVICE double sum_list(int count, size_t_ size) {
-    double sum = 0;
-    #pragma unroll
-    for(int i = 0; i < each_list; ++i) {
-      int e = tid * each_list + i;
-      sum += e < count ? size(e) : 0.0;
-    }
-    return fold_sum(sum);
+    found = cta_min(found);
+    any = cta_max(any);
+    return 0xffffffffu != found ? (int)found : (int)any - 1;
   }
 
-  // The first CTA alone: the list holds every token that may be kept, `total`
-  // is the weight that top-p refers to (below 0: the list's first `count`).
+  // The first CTA alone: the sorted list's first `count` entries are all tokens
+  // that may be kept, `total` is the weight that top-p refers to (below 0: that
+  // of these entries).
   MGPU_DEVICE int finish_list(int count, double total, float top_p, float min_p,
     double u) {
-    auto by_place = [&](int e) { return weight(key_value(list_key(e))); };
+    for(int e = tid; e < count; e += nt)
+      shared.list_weights[e] = weight(key_value(list_key(e)));
+    __syncthreads();
+    if(count <= 128) {
+      if(!warp) {
+        int token = finish_short(count, total, top_p, min_p, u);
+        if(!lane) shared.hit = token;
+      }
+      __syncthreads();
+      return shared.hit;
+    }
+    auto by_place = [&](int e) { return shared.list_weights[e]; };
     if(top_p < 1) {
-      if(total < 0) total = sum_list(count, by_place);
+      if(total < 0) {
+        double sum = 0;
+        for(int e = tid; e < count; e += nt) sum += by_place(e);
+        total = cta_sum(sum);
+      }
       double target = (double)top_p * total;
       count = search_list(count, by_place,
         [&](double sum) { return sum >= target; }) + 1;
     }
     if(min_p > 0) {
       // Weights fall along the list.
-      int fit = 0;
+      uint32_t fit = 0;
       for(int e = tid; e < count; e += nt)
         if(list_key(e) == peak_key || by_place(e) >= (double)min_p) fit = e + 1;
-      count = fold_max(fit);
+      count = (int)cta_max(fit);
     }
-    if(count < 2) return list_index(0);
     // By index, with the key in the low half.
     for(int e = tid; e < count; e += nt) {
-      unsigned long long entry = shared.list[e];
-      shared.list[e] = entry << 32 | entry >> 32;
+      unsigned long long old = shared.list[e];
+      shared.list[e] = old << 32 | old >> 32;
     }
     sort_list(count);
-    auto by_index = [&](int e) {
-      return weight(key_value((uint32_t)shared.list[e]));
-    };
-    double target = u * sum_list(count, by_index);
-    int e = search_list(count, by_index,
+    double sum = 0;
+    for(int e = tid; e < count; e += nt) {
+      shared.list_weights[e] = weight(key_value((uint32_t)shared.list[e]));
+      sum += shared.list_weights[e];
+    }
+    double target = u * cta_sum(sum);
+    int e = search_list(count, by_place,
       [&](double sum) { return sum > target; });
     return (int)(0xffffffffu - (uint32_t)(shared.list[e] >> 32));
+  }
+  // The same for at most 128 entries, by one warp with four to a lane. The draw
+  // adds up, for each entry, those of no higher index.
+  MGPU_DEVICE int finish_short(int count, double total, float top_p,
+    float min_p, double u) {
+    double own[4], sum = 0;
+    #pragma unroll
+    for(int i = 0; i < 4; ++i) {
+      int e = lane * 4 + i;
+      own[i] = e < count ? shared.list_weights[e] : 0.0;
+      sum += own[i];
+    }
+    if(top_p < 1) {
+      double at = upto(sum);
+      if(total < 0) total = __shfl_sync(0xffffffffu, at, 31);
+      double target = (double)top_p * total;
+      at -= sum;
+      uint32_t found = 0xffffffffu, any = 0;
+      #pragma unroll
+      for(int i = 0; i < 4; ++i) {
+        at += own[i];
+        if(own[i] > 0) {
+          any = lane * 4 + i + 1;
+          if(0xffffffffu == found && at >= target) found = any;
+        }
+      }
+      found = __reduce_min_sync(0xffffffffu, found);
+      any = __reduce_max_sync(0xffffffffu, any);
+      count = (int)(0xffffffffu != found ? found : any);
+    }
+    if(min_p > 0) {
+      uint32_t fit = 0;
+      #pragma unroll
+      for(int i = 0; i < 4; ++i) {
+        int e = lane * 4 + i;
+        if(e < count && (list_key(e) == peak_key || own[i] >= (double)min_p))
+          fit = e + 1;
+      }
+      count = (int)__reduce_max_sync(0xffffffffu, fit);
+    }
+    double upto_mine[4] = { 0, 0, 0, 0 };
+    sum = 0;
+    for(int q = 0; q < count; ++q) {
+      double w = shared.list_weights[q];
+      int at = list_index(q);
+      sum += w;
+      #pragma unroll
+      for(int i = 0; i < 4; ++i) {
+        int e = lane * 4 + i;
+        if(e < count && at <= list_index(e)) upto_mine[i] += w;
+      }
+    }
+    double target = u * sum;
+    uint32_t hit = 0xffffffffu, any = 0;
+    #pragma unroll
+    for(int i = 0; i < 4; ++i) {
+      int e = lane * 4 + i;
+      if(e < count && own[i] > 0) {
+        uint32_t at = (uint32_t)list_index(e);
+        any = max(any, at);
+        if(upto_mine[i] > target) hit = min(hit, at);
+      }
+    }
+    hit = __reduce_min_sync(0xffffffffu, hit);
+    any = __reduce_max_sync(0xffffffffu, any);
+    return (int)(0xffffffffu != hit ? hit : any);
+  }
+
+  //////////////////////////////////////////////////////////////////////////////
+  // Top-k of few tokens. Instead of a common histogram every CTA takes one of
+  // its own part, from its own peak down, and lists what may be among the row's
+  // greatest. The row's peak key is known behind it. True where the first CTA's
+  // list, `listed` long, holds the greatest top_k; false where a part has too
+  // many equal tokens for its share of the list.
+  MGPU_DEVICE bool list_greatest(int top_k, int& listed) {
+    uint32_t part_key = cta_max(part_peak());
+    float from = key_value(part_key);
+    bool some = part_key != 0xffffffffu && from > -INFINITY;
+    clear_hist();
+    auto step = [&](float value) {
+      float d = value == from ? 0.0f : (from - value) * inv_temperature;
+      return bin(d);
+    };
+    if(some)
+      each([&](float value, int) { atomicAdd(&shared.hist[step(value)], 1u); });
+    __syncthreads();
+    // The step in which the count reaches top_k.
+    enum { most = sample_bins / nt };
+    int counts[most], sum = 0;
+    #pragma unroll
+    for(int i = 0; i < most; ++i) {
+      counts[i] = (int)shared.hist[tid * most + i];
+      sum += counts[i];
+    }
+    int at = (int)cta_upto((double)sum) - sum;
+    uint32_t border = sample_bins - 1, taken = 0;
+    #pragma unroll
+    for(int i = 0; i < most; ++i) {
+      at += counts[i];
+      if(at >= top_k && border == sample_bins - 1) {
+        border = tid * most + i;
+        taken = at;
+      }
+    }
+    border = cta_min(border);
+    // What is in the steps up to it: the count of the thread that has it, or
+    // all.
+    bool has = (int)border / most == tid && taken;
+    uint32_t in_list = cta_max(has ? taken : 0);
+    uint32_t all = cta_max(tid == nt - 1 ? (uint32_t)at : 0);
+    if(border == sample_bins - 1) in_list = all;
+    sample_news_t mine = { };
+    mine.p = part_key;
+    mine.i = (int)in_list;
+    const sample_news_t* news = share(mine);
+    uint32_t key = 0;
+    int before = 0, total = 0;
+    bool fits = true;
+    for(int r = 0; r < ctas; ++r) {
+      key = max(key, news[r * warps].p);
+      if(r == rank) before = total;
+      total += news[r * warps].i;
+    }
+    fits = total <= sample_list;
+    peak_key = key;
+    listed = total;
+    if(!fits || 0xffffffffu == key) return fits;
+    if(!tid) shared.list_count = before;
+    __syncthreads();
+    if(some) {
+      shared_t* first = cluster.map_shared_rank(&shared, 0);
+      each([&](float value, int v) {
+        if(step(value) <= (int)border) {
+          int to = atomicAdd(&shared.list_count, 1);
+          if(to < sample_list) first->list[to] = entry(order_key(value), v);
+        }
+      });
+    }
+    cluster.sync();
+    if(!tid) shared.list_count = 0;
+    return true;
   }
 
   //////////////////////////////////////////////////////////////////////////////
@@ -652,7 +858,7 @@ struct sample_cta_t {
     bool list = whole || band.inside <= 1.25 * sample_list;
     double above = 0, all = 0;
     uint32_t low = 0xffffffffu, high = 0;
-    int inside = 0;
+    int inside = 0, appended = 0;
     each([&](float value, int v) {
       uint32_t key = order_key(value);
       if(!kept(key, v)) return;
@@ -663,40 +869,53 @@ struct sample_cta_t {
       if(b > band.hi) return;
       if(b < band.lo) {
         above += w;
-        if(whole) append(key, v);
+        if(whole) {
+          append(key, v);
+          ++appended;
+        }
       } else {
         ++inside;
         low = min(low, key);
         high = max(high, key);
-        if(list) append(key, v);
+        if(list) {
+          append(key, v);
+          ++appended;
+        }
       }
     });
     sample_news_t mine = { };
-    mine.a = fold_sum(above);
-    mine.b = fold_sum(all);
-    mine.p = ~fold_max(~low);
-    mine.q = fold_max(high);
-    mine.i = (int)fold_sum((double)inside);
+    mine.a = warp_sum(above);
+    mine.b = warp_sum(all);
+    mine.p = __reduce_min_sync(0xffffffffu, low);
+    mine.q = __reduce_max_sync(0xffffffffu, high);
+    mine.i = __reduce_add_sync(0xffffffffu, inside);
+    mine.j = __reduce_add_sync(0xffffffffu, appended);
     const sample_news_t* news = share(mine);
     above = all = 0;
     low = 0xffffffffu;
     high = 0;
-    inside = 0;
-    for(int r = 0; r < ctas; ++r) {
-      above += news[r].a;
-      all += news[r].b;
-      low = min(low, news[r].p);
-      high = max(high, news[r].q);
-      inside += news[r].i;
-    }
+    inside = appended = 0;
+    all_news(news, [&](const sample_news_t& n) {
+      above += n.a;
+      all += n.b;
+      low = min(low, n.p);
+      high = max(high, n.q);
+      inside += n.i;
+      appended += n.j;
+    });
+    above = warp_sum(above);
+    all = warp_sum(all);
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    inside = __reduce_add_sync(0xffffffffu, inside);
+    appended = __reduce_add_sync(0xffffffffu, appended);
     total = all;
+    listed = appended;
     if(!by_count) target *= all;
-    if(whole) {
-      listed = min(shared.list_count, (int)sample_list);   // the first CTA's
-      return true;
-    }
+    // Holds by the bound on the steps' tokens; else the border is looked for.
+    if(whole && appended <= sample_list) return true;
+    list = list && !whole && appended <= sample_list;
 
-    list = list && inside <= sample_list;
     while(inside > sample_list && low < high) {
       uint32_t middle = low + (high - low) / 2;
       double upper = 0;
@@ -713,21 +932,25 @@ struct sample_cta_t {
           lower_high = max(lower_high, key);
       });
       mine = sample_news_t { };
-      mine.a = fold_sum(upper);
-      mine.p = ~fold_max(~upper_low);
-      mine.q = fold_max(lower_high);
-      mine.i = (int)fold_sum((double)upper_count);
+      mine.a = warp_sum(upper);
+      mine.p = __reduce_min_sync(0xffffffffu, upper_low);
+      mine.q = __reduce_max_sync(0xffffffffu, lower_high);
+      mine.i = __reduce_add_sync(0xffffffffu, upper_count);
       news = share(mine);
       upper = 0;
       upper_low = 0xffffffffu;
       lower_high = 0;
       upper_count = 0;
-      for(int r = 0; r < ctas; ++r) {
-        upper += news[r].a;
-        upper_low = min(upper_low, news[r].p);
-        lower_high = max(lower_high, news[r].q);
-        upper_count += news[r].i;
-      }
+      all_news(news, [&](const sample_news_t& n) {
+        upper += n.a;
+        upper_low = min(upper_low, n.p);
+        lower_high = max(lower_high, n.q);
+        upper_count += n.i;
+      });
+      upper = warp_sum(upper);
+      upper_low = __reduce_min_sync(0xffffffffu, upper_low);
+      lower_high = __reduce_max_sync(0xffffffffu, lower_high);
+      upper_count = __reduce_add_sync(0xffffffffu, upper_count);
       if(above + upper >= target) {
         low = upper_low;
         inside = upper_count;
@@ -737,7 +960,7 @@ struct sample_cta_t {
         inside -= upper_count;
       }
     }
-    if(inside > sample_list) {
+    if(inside > sample_list || low == high) {
       // One value: as many of its tokens as it takes.
       double need = ceil((target - above) / size<by_count>(key_value(low)));
       need = need > 1 ? (need < vocabulary ? need : vocabulary) : 1;
@@ -784,13 +1007,12 @@ struct sample_cta_t {
     };
     double sum = 0;
     each([&](float value, int v) { sum += left(value, v); });
-    #pragma unroll
-    for(int offset = 16; offset; offset /= 2)
-      sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    share_run_sum(sum);
-    double target = u * total_of_runs(), before = 0;
+    sample_news_t mine = { };
+    mine.a = warp_sum(sum);
+    const sample_news_t* news = share(mine);
+    double target = u * total_of_runs(news), before = 0;
     auto test = [&](double s) { return s > target; };
-    int found = find_run(test, before);
+    int found = find_run(news, test, before);
     if(found >= 0 && found / warps == rank) {
       int at = search_run(found, before, left, test);
       if(!tid) *token = at;
@@ -816,33 +1038,39 @@ sample_k(const real_t* logits, int64_t stride, int vocabulary,
   sample_cta_t<nt, real_t> cta(logits + at * stride, vocabulary, shared);
   bool leader = !cta.rank && !cta.tid;
   if(!cta.tid) shared.list_count = 0;
-  cta.peak_key = cta.find_peak();
+  cta.make_powers();
+  cta.log2_scale = 1.4426950408889634 / (double)temperature;
+  cta.inv_temperature = 1.0f / temperature;
+  // A part's list holds its greatest top_k and its border's equals.
+  bool by_k = temperature > 0 && top_k > 0 && top_k < vocabulary;
+  bool listed = false, peaked = false;
+  double total = -1;
+  int count = 0;
+  if(by_k && top_k * ctas <= sample_list / 2) {
+    listed = cta.list_greatest(top_k, count);
+    peaked = true;
+  }
+  if(!peaked) cta.find_peak();
   cta.peak = key_value(cta.peak_key);
-  // A NaN has the greatest key of all.
   if(0xffffffffu == cta.peak_key || !(cta.peak > -INFINITY)) {
     if(leader) tokens[at] = -1;
   } else if(!(temperature > 0)) {
     int first = cta.first_of(cta.peak_key);
     if(leader) tokens[at] = first;
   } else {
-    cta.scale = 1.0 / (double)temperature;
-    cta.inv_temperature = 1.0f / temperature;
-    bool listed = false;
-    double total = -1;
-    int count = 0;
-    if(top_k > 0 && top_k < vocabulary) {
+    if(by_k && !listed) {
       listed = cta.template find_border<true>((double)top_k, total, count);
       // The weight that top-p refers to is that of the first top_k.
       total = -1;
     }
-    bool by_k = listed;
+    bool first_k = listed;
     if(!listed && top_p < 1)
       listed = cta.template find_border<false>((double)top_p, total, count);
     if(!listed)
       cta.draw(min_p, u, tokens + at);
     else if(!cta.rank) {
       cta.sort_list(count);
-      int token = cta.finish_list(by_k ? min(count, top_k) : count, total,
+      int token = cta.finish_list(first_k ? min(count, top_k) : count, total,
         top_p, min_p, u);
       if(!cta.tid) tokens[at] = token;
     }
