@@ -104,9 +104,9 @@ struct sample_shared_t {
   int list_count, hit;
 };
 
-template<int nt, typename real_t>
+template<int nt, bool staged, typename real_t>
 struct sample_cta_t {
-  enum { warps = nt / 32, pack = 16 / (int)sizeof(real_t),
+  enum { warps = nt / 32, pack = 16 / (int)sizeof(real_t), batch = 4,
     each_list = sample_list / nt, runs = sample_max_cluster * warps,
     each_lane = runs / 32 };
   typedef pack_t<real_t, pack> word_t;
@@ -114,22 +114,27 @@ struct sample_cta_t {
   struct band_t { int lo, hi; double tokens, inside; };
 
   const real_t* x;
+  word_t* stage;       // the CTA's part, where it fits into shared memory
   int vocabulary;
   shared_t& shared;
   cooperative_groups::cluster_group cluster;
   int rank, ctas, tid, lane, warp, run;
-  int64_t run_begin, run_end;     // in elements behind the row's 16-byte border
+  // In elements behind the row's 16-byte border.
+  int64_t part_begin, run_begin, run_end;
   int shift;                      // where on it the row begins
   int exchanges;
 
-  float peak, inv_temperature;
+  float peak, steps_per_logit;
   uint32_t peak_key;
   double log2_scale;   // log2(e) / T
+  float weightless;    // logits below have no weight
+  double run_left;     // see find_border
   uint32_t least;      // what is kept: keys above this one,
   int last;            // and those equal to it up to this index
 
-  MGPU_DEVICE sample_cta_t(const real_t* x_, int vocabulary_,
-    shared_t& shared_) : x(x_), vocabulary(vocabulary_), shared(shared_),
+  MGPU_DEVICE sample_cta_t(const real_t* x_, word_t* stage_, int vocabulary_,
+    shared_t& shared_) : x(x_), stage(stage_), vocabulary(vocabulary_),
+    shared(shared_),
     cluster(cooperative_groups::this_cluster()),
     rank((int)cluster.block_rank()), ctas((int)cluster.num_blocks()),
     tid((int)threadIdx.x), lane((int)threadIdx.x % 32),
@@ -137,6 +142,7 @@ struct sample_cta_t {
     run = rank * warps + warp;
     shift = (int)((uintptr_t)x % 16 / sizeof(real_t));
     int64_t end = (int64_t)vocabulary + shift, length = run_length();
+    part_begin = length * rank * warps;
     run_begin = min(length * run, end);
     run_end = min(run_begin + length, end);
   }
@@ -146,44 +152,88 @@ struct sample_cta_t {
       step) * step;
   }
 
-  // f(logit, index) for the tokens of this warp's run.
-  template<typename func_t>
-  MGPU_DEVICE __forceinline__ void each(func_t f) const {
-    enum { ahead = pack == 4 ? 4 : 2, step = 32 * pack };
-    int64_t a = run_begin + lane * pack;
-    // Whole words, some of them in flight at a time, then the ragged ends.
-    if(a < shift) {
-      some(a, f);
-      a += step;
+  // The word at element a of the row itself; -infinity outside of it, which has
+  // no weight and is never drawn.
+  MGPU_DEVICE __forceinline__ word_t load(int64_t a) const {
+    word_t word;
+    if(a >= shift && a + pack <= run_end)
+      word = *(const word_t*)(x + (a - shift));
+    else {
+      #pragma unroll
+      for(int j = 0; j < pack; ++j)
+        word.v[j] = a + j >= shift && a + j < run_end ? x[a + j - shift] :
+          from_f32<real_t>(-INFINITY);
     }
-    for(; a + ((ahead - 1) * step + pack) <= run_end; a += ahead * step) {
-      const real_t* from = x + (a - shift);
+    return word;
+  }
+  MGPU_DEVICE __forceinline__ float logit_at(int64_t a) const {
+    return to_f32(staged ? ((const real_t*)stage)[a - part_begin] :
+      x[a - shift]);
+  }
+
+  // The first pass: the run's greatest logit as a key, a NaN's the greatest of
+  // all; where there is room the run moves into shared memory, because a barrier
+  // of the cluster empties the L1. Several words are in flight.
+  MGPU_DEVICE uint32_t part_peak() const {
+    enum { ahead = 4, step = 32 * pack };
+    float peak = -INFINITY;
+    for(int64_t a = run_begin + lane * pack; a < run_end; a += ahead * step) {
       word_t words[ahead];
       #pragma unroll
       for(int i = 0; i < ahead; ++i)
-        words[i] = *(const word_t*)(from + i * step);
+        if(a + i * step < run_end) words[i] = load(a + i * step);
       #pragma unroll
       for(int i = 0; i < ahead; ++i)
-        #pragma unroll
-        for(int j = 0; j < pack; ++j)
-          f(to_f32(words[i].v[j]), (int)(a - shift) + i * step + j);
+        if(a + i * step < run_end) {
+          if(staged) stage[(a - part_begin) / pack + i * 32] = words[i];
+          #pragma unroll
+          for(int j = 0; j < pack; ++j)
+            peak = max_or_nan(peak, to_f32(words[i].v[j]));
+        }
     }
-    for(; a < run_end; a += step) {
-      if(a + pack <= run_end) {
-        word_t word = *(const word_t*)(x + (a - shift));
-        #pragma unroll
-        for(int j = 0; j < pack; ++j)
-          f(to_f32(word.v[j]), (int)(a - shift) + j);
-      } else
-        some(a, f);
-    }
+    uint32_t key = isnan(peak) ? 0xffffffffu : order_key(peak);
+    __syncwarp();
+    return __reduce_max_sync(0xffffffffu, run_begin < run_end ? key : 0u);
   }
+  MGPU_DEVICE static float max_or_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+  }
+
+  // f(logits, index of the first) for four neighbouring tokens of this warp's
+  // run at a time. One copy of f's code for every part of a word: these passes
+  // run once, and wait for instructions where they are long.
   template<typename func_t>
-  MGPU_DEVICE __forceinline__ void some(int64_t a, func_t f) const {
-    int64_t begin = max(a, (int64_t)shift), end = min(a + pack, run_end);
-    for(int64_t i = begin; i < end; ++i)
-      f(to_f32(x[i - shift]), (int)(i - shift));
+  MGPU_DEVICE __forceinline__ void each_four(func_t f) const {
+    enum { step = 32 * pack };
+    int64_t a = run_begin + lane * pack;
+    if(a >= run_end) return;
+    word_t next = staged ? stage[(a - part_begin) / pack] : load(a);
+    #pragma unroll 1
+    for(; a < run_end; a += step) {
+      word_t word = next;
+      if(a + step < run_end)
+        next = staged ? stage[(a + step - part_begin) / pack] : load(a + step);
+      #pragma unroll
+      for(int h = 0; h < pack; h += batch) {
+        float logits[batch];
+        #pragma unroll
+        for(int j = 0; j < batch; ++j) logits[j] = to_f32(word.v[h + j]);
+        f(logits, (int)(a - shift) + h);
+      }
+    }
   }
+  // f(logit, index) for the tokens of this warp's run.
+  template<typename func_t>
+  MGPU_DEVICE __forceinline__ void each(func_t f) const {
+    each_four([&](const float (&logits)[batch], int v) {
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) f(logits[j], v + j);
+    });
+  }
+  // Whether no token has been dropped so far.
+  MGPU_DEVICE bool all_kept() const { return 0 == least; }
 
   //////////////////////////////////////////////////////////////////////////////
   // Sums.
@@ -268,9 +318,9 @@ struct sample_cta_t {
   // at most 1/128 in size, it is 2^(i / 64) 2^r: a power from the table and the
   // Taylor series of exp(r ln 2), whose sixth-degree term is below 4e-17. Eleven
   // operations of 64 bits; the library's exp takes several times as many, and
-  // these passes are bound by them. Below 2^-1000 it is 0.
+  // these passes are bound by instructions. Below about 2^-1000 it is 0.
   MGPU_DEVICE double weight(float value) const {
-    if(value == peak) return 1.0;
+    if(peak == INFINITY) return value == peak ? 1.0 : 0.0;
     const double magic = 1.5 * 70368744177664.0;       // 1.5 * 2^46: ulp 2^-6
     double d = (double)value - (double)peak;
     double z = fma(d, log2_scale, magic);
@@ -284,31 +334,28 @@ struct sample_cta_t {
     p = fma(p, r, 6.931471805599453e-1);
     double t = shared.powers[i & (sample_powers - 1)];
     t = fma(t, p * r, t);
-    int exponent = i >> 6;
-    double w = __hiloint2double(__double2hiint(t) + exponent * (1 << 20),
-      __double2loint(t));
-    return d * log2_scale < -1000.0 ? 0.0 : w;
+    double w = __hiloint2double(__double2hiint(t) +
+      (i & ~(sample_powers - 1)) * (1 << 14), __double2loint(t));
+    return value < weightless ? 0.0 : w;
   }
   template<bool by_count>
   MGPU_DEVICE double size(float value) const {
     return by_count ? 1.0 : weight(value);
   }
-  // Neither rises where the logit does.
-  MGPU_DEVICE float distance(float value) const {
-    return value == peak ? 0.0f : (peak - value) * inv_temperature;
+  // The distance from the peak in steps, at most the last one; it does not rise
+  // where the logit does. The step is the nearest whole number.
+  MGPU_DEVICE float steps_below(float from, float value) const {
+    if(from == INFINITY) return value == from ? 0.0f : sample_bins - 1.0f;
+    return fminf((from - value) * steps_per_logit, sample_bins - 1.0f);
   }
-  MGPU_DEVICE int bin(float distance) const {
-    return (int)fminf(distance * (float)sample_steps, sample_bins - 1.0f);
+  MGPU_DEVICE static float rounder() { return 12582912.0f; }   // 1.5 * 2^23
+  MGPU_DEVICE static int nearest(float rounded) {
+    return __float_as_int(rounded) - 0x4b400000;
+  }
+  MGPU_DEVICE int bin(float value) const {
+    return nearest(steps_below(peak, value) + rounder());
   }
 
-  // A NaN has the greatest key of all.
-  MGPU_DEVICE uint32_t part_peak() const {
-    uint32_t key = 0;
-    each([&](float value, int) {
-      key = max(key, isnan(value) ? 0xffffffffu : order_key(value));
-    });
-    return __reduce_max_sync(0xffffffffu, key);
-  }
   MGPU_DEVICE void find_peak() {
     sample_news_t mine = { };
     mine.p = part_peak();
@@ -394,7 +441,7 @@ struct sample_cta_t {
     int64_t part_end = min(part_begin + part, end);
     double sum = 0;
     for(int64_t a = part_begin + lane; a < part_end; a += 32)
-      if(a >= shift) sum += size(to_f32(x[a - shift]), (int)(a - shift));
+      if(a >= shift) sum += size(logit_at(a), (int)(a - shift));
     sum = warp_sum(sum);
     if(!lane) shared.fold[0][warp] = sum;
     if(!tid) shared.hit = -1;
@@ -417,7 +464,7 @@ struct sample_cta_t {
       for(int64_t first = part_begin; first < part_end && !done; first += 32) {
         int64_t a = first + lane;
         double own = a >= shift && a < part_end ?
-          size(to_f32(x[a - shift]), (int)(a - shift)) : 0.0;
+          size(logit_at(a), (int)(a - shift)) : 0.0;
         double sum = upto(own);
         unsigned some = __ballot_sync(0xffffffffu, own > 0);
         unsigned hits = __ballot_sync(0xffffffffu, own > 0 && test(before + sum));
@@ -465,6 +512,7 @@ struct sample_cta_t {
 
   MGPU_DEVICE void clear_hist() {
     for(int b = tid; b < sample_bins; b += nt) shared.hist[b] = 0;
+    if(!tid) shared.list_count = 0;
     __syncthreads();
   }
 
@@ -473,18 +521,18 @@ struct sample_cta_t {
     // Fixed-point weights: a step's sum stays below 2^32 whatever it holds.
     float unit = by_count ? 1.0f : fminf(4096.0f, 2147483648.0f / vocabulary);
     clear_hist();
+    bool every = all_kept();
     each([&](float value, int v) {
-      if(!kept(order_key(value), v)) return;
-      float d = distance(value);
-      int b = bin(d);
+      float s = steps_below(peak, value), rounded = s + rounder();
       uint32_t add = 1;
       if(!by_count) {
-        // exp(-f) for 0 <= f <= 1 / 64, to 1e-6.
-        float f = fminf(fmaxf(d - b * (1.0f / sample_steps), 0.0f),
-          1.0f / sample_steps);
-        add = (uint32_t)__float2int_rn(unit * (1.0f - f + 0.5f * f * f));
+        // exp(-r / 64) for |r| <= 1/2, to 1e-7.
+        float r = s - (rounded - rounder());
+        add = __float_as_uint(fmaf(r, fmaf(r, unit / 8192, -unit / 64), unit) +
+          8388608.0f) & 0x7fffff;
       }
-      atomicAdd(&shared.hist[b], add);
+      if(every || kept(order_key(value), v))
+        atomicAdd(&shared.hist[nearest(rounded)], add);
     });
     if(!tid) {
       shared.band_lo = shared.band_hi = sample_bins;
@@ -500,7 +548,7 @@ struct sample_cta_t {
     int first = rank * slice + tid * each_thread;
     double weights[most], tokens[most], weight_sum = 0, token_sum = 0;
     // A token adds at least this much.
-    double fewest = by_count ? 1.0 : (double)unit * 0.984 - 0.5;
+    double fewest = by_count ? 1.0 : (double)unit * 0.992 - 0.5;
     #pragma unroll
     for(int i = 0; i < most; ++i) {
       weights[i] = tokens[i] = 0;
@@ -595,10 +643,40 @@ struct sample_cta_t {
   MGPU_DEVICE static unsigned long long entry(uint32_t key, int v) {
     return (unsigned long long)key << 32 | (0xffffffffu - v);
   }
+  // Each CTA appends to a list of its own; the first one fetches them.
   MGPU_DEVICE void append(uint32_t key, int v) {
-    shared_t* first = cluster.map_shared_rank(&shared, 0);
-    int at = atomicAdd(&first->list_count, 1);
-    if(at < sample_list) first->list[at] = entry(key, v);
+    int at = atomicAdd(&shared.list_count, 1);
+    if(at < sample_list) shared.list[at] = entry(key, v);
+  }
+  // For at most sample_list entries in all, behind a barrier of the cluster. The
+  // others keep their lists until they have passed another one. The histogram's
+  // memory is free by now.
+  MGPU_DEVICE void fetch_lists() {
+    unsigned long long* all = (unsigned long long*)shared.hist;
+    int counts[sample_max_cluster], count = 0;
+    #pragma unroll
+    for(int r = 0; r < sample_max_cluster; ++r)
+      counts[r] = r < ctas ?
+        min(cluster.map_shared_rank(&shared, r)->list_count, (int)sample_list) :
+        0;
+    #pragma unroll
+    for(int r = 0; r < sample_max_cluster; ++r) {
+      for(int i = tid; i < counts[r]; i += nt)
+        if(count + i < sample_list)
+          all[count + i] = cluster.map_shared_rank(&shared, r)->list[i];
+      count += counts[r];
+    }
+    // The first CTA's own entries stay in front, in its weights' memory.
+    unsigned long long* own = (unsigned long long*)shared.list_weights;
+    for(int i = tid; i < counts[0]; i += nt) own[i] = shared.list[i];
+    __syncthreads();
+    for(int i = tid; i < count && i < sample_list; i += nt)
+      shared.list[i] = all[i];
+    __syncthreads();
+  }
+  // The CTA's own list behind fetch_lists.
+  MGPU_DEVICE const unsigned long long* own_list() const {
+    return rank ? shared.list : (unsigned long long*)shared.list_weights;
   }
   MGPU_DEVICE uint32_t list_key(int i) const {
     return (uint32_t)(shared.list[i] >> 32);
@@ -783,8 +861,7 @@ struct sample_cta_t {
     bool some = part_key != 0xffffffffu && from > -INFINITY;
     clear_hist();
     auto step = [&](float value) {
-      float d = value == from ? 0.0f : (from - value) * inv_temperature;
-      return bin(d);
+      return nearest(steps_below(from, value) + rounder());
     };
     if(some)
       each([&](float value, int) { atomicAdd(&shared.hist[step(value)], 1u); });
@@ -842,50 +919,74 @@ struct sample_cta_t {
       });
     }
     cluster.sync();
-    if(!tid) shared.list_count = 0;
     return true;
   }
 
   //////////////////////////////////////////////////////////////////////////////
   // Pass 3 and what follows from it: `least` and `last` for the tokens above
   // the border. True where the list holds all that is left; the weight of what
-  // was kept before is in `total`, the list's length in `listed`.
+  // was kept before is in `total`, the list's length in `listed`. Where it is known
+  // at the end what is left in each run, it is in run_left, and `drawable` is set.
 
   template<bool by_count>
-  MGPU_DEVICE bool find_border(double target, double& total, int& listed) {
+  MGPU_DEVICE bool find_border(double target, float min_p, double& total,
+    int& listed, bool& drawable) {
     band_t band = find_band<by_count>(target);
     bool whole = band.tokens <= sample_list;
     bool list = whole || band.inside <= 1.25 * sample_list;
-    double above = 0, all = 0;
+    double above = 0, all = 0, left = 0;
     uint32_t low = 0xffffffffu, high = 0;
     int inside = 0, appended = 0;
-    each([&](float value, int v) {
-      uint32_t key = order_key(value);
-      if(!kept(key, v)) return;
-      int b = bin(distance(value));
-      if(by_count && b > band.hi) return;
-      double w = size<by_count>(value);
-      all += w;
-      if(b > band.hi) return;
-      if(b < band.lo) {
+    bool every = all_kept();
+    each_four([&](const float (&logits)[batch], int v) {
+      // Without branches between the four, so that their chains of dependent
+      // 64-bit operations overlap.
+      bool live[batch], some = false;
+      int bins[batch];
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) {
+        bins[j] = bin(logits[j]);
+        live[j] = every || kept(order_key(logits[j]), v + j);
+        if(by_count) live[j] = live[j] && bins[j] <= band.hi;
+        some = some || live[j];
+      }
+      if(!some) return;
+      double weights[batch];
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) weights[j] = size<by_count>(logits[j]);
+      bool listed = false;
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) {
+        double w = live[j] ? weights[j] : 0.0;
+        live[j] = live[j] && bins[j] <= band.hi;
+        bool in = live[j] && bins[j] >= band.lo;
+        all += w;
+        w = bins[j] < band.lo ? w : 0.0;
         above += w;
-        if(whole) {
-          append(key, v);
-          ++appended;
-        }
-      } else {
-        ++inside;
-        low = min(low, key);
-        high = max(high, key);
-        if(list) {
-          append(key, v);
-          ++appended;
-        }
+        if(!by_count && min_p > 0)
+          left += w >= (double)min_p || logits[j] == peak ? w : 0.0;
+        inside += in;
+        live[j] = whole ? live[j] : in;
+        listed = listed || live[j];
+      }
+      if(listed) {
+        #pragma unroll
+        for(int j = 0; j < batch; ++j)
+          if(live[j]) {
+            uint32_t key = order_key(logits[j]);
+            low = min(low, key);
+            high = max(high, key);
+            if(list) {
+              append(key, v + j);
+              ++appended;
+            }
+          }
       }
     });
     sample_news_t mine = { };
     mine.a = warp_sum(above);
     mine.b = warp_sum(all);
+    run_left = !by_count && min_p > 0 ? warp_sum(left) : mine.a;
     mine.p = __reduce_min_sync(0xffffffffu, low);
     mine.q = __reduce_max_sync(0xffffffffu, high);
     mine.i = __reduce_add_sync(0xffffffffu, inside);
@@ -913,7 +1014,11 @@ struct sample_cta_t {
     listed = appended;
     if(!by_count) target *= all;
     // Holds by the bound on the steps' tokens; else the border is looked for.
-    if(whole && appended <= sample_list) return true;
+    if(whole && appended <= sample_list) {
+      if(!rank) fetch_lists();
+      cluster.sync();
+      return true;
+    }
     list = list && !whole && appended <= sample_list;
 
     while(inside > sample_list && low < high) {
@@ -964,15 +1069,14 @@ struct sample_cta_t {
       // One value: as many of its tokens as it takes.
       double need = ceil((target - above) / size<by_count>(key_value(low)));
       need = need > 1 ? (need < vocabulary ? need : vocabulary) : 1;
-      if(!rank && !tid) shared.list_count = 0;   // behind the appends' barrier
       int at = nth_equal(low, need);
       least = low;
       last = at;
       return false;
     }
     if(!list) {
-      if(!rank && !tid) shared.list_count = 0;
-      cluster.sync();
+      if(!tid) shared.list_count = 0;
+      __syncthreads();
       each([&](float value, int v) {
         uint32_t key = order_key(value);
         if(key >= low && key <= high && kept(key, v)) append(key, v);
@@ -980,7 +1084,9 @@ struct sample_cta_t {
       cluster.sync();
     }
     mine = sample_news_t { };
+    int own_listed = shared.list_count;
     if(!rank) {
+      fetch_lists();
       sort_list(inside);
       int e = search_list(inside, [&](int e) {
           return size<by_count>(key_value(list_key(e)));
@@ -988,17 +1094,30 @@ struct sample_cta_t {
       e = max(e, 0);
       mine.p = list_key(e);
       mine.i = list_index(e);
-      __syncthreads();
-      if(!tid) shared.list_count = 0;
     }
     news = share(mine);
     least = news[0].p;
     last = news[0].i;
+    if(list && !by_count) {
+      // Of the steps at the border only the listed tokens matter.
+      int64_t length = run_length();
+      double sum = 0;
+      for(int i = lane; i < own_listed; i += 32) {
+        unsigned long long e = own_list()[i];
+        uint32_t key = (uint32_t)(e >> 32);
+        int v = (int)(0xffffffffu - (uint32_t)e);
+        double w = weight(key_value(key));
+        if((v + (int64_t)shift) / length == run && kept(key, v) &&
+          (w >= (double)min_p || key == peak_key)) sum += w;
+      }
+      run_left += warp_sum(sum);
+      drawable = true;
+    }
     return false;
   }
 
   // Pass 4.
-  MGPU_DEVICE void draw(float min_p, double u, int* token) {
+  MGPU_DEVICE void draw(float min_p, double u, bool drawable, int* token) {
     auto left = [&](float value, int v) {
       uint32_t key = order_key(value);
       if(!kept(key, v)) return 0.0;
@@ -1006,9 +1125,27 @@ struct sample_cta_t {
       return w >= (double)min_p || key == peak_key ? w : 0.0;
     };
     double sum = 0;
-    each([&](float value, int v) { sum += left(value, v); });
+    bool every = all_kept();
+    if(!drawable) each_four([&](const float (&logits)[batch], int v) {
+      bool live[batch], some = false;
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) {
+        live[j] = every || kept(order_key(logits[j]), v + j);
+        some = some || live[j];
+      }
+      if(!some) return;
+      double weights[batch];
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) weights[j] = weight(logits[j]);
+      #pragma unroll
+      for(int j = 0; j < batch; ++j) {
+        live[j] = live[j] &&
+          (weights[j] >= (double)min_p || logits[j] == peak);
+        sum += live[j] ? weights[j] : 0.0;
+      }
+    });
     sample_news_t mine = { };
-    mine.a = warp_sum(sum);
+    mine.a = drawable ? run_left : warp_sum(sum);
     const sample_news_t* news = share(mine);
     double target = u * total_of_runs(news), before = 0;
     auto test = [&](double s) { return s > target; };
@@ -1020,10 +1157,11 @@ struct sample_cta_t {
   }
 };
 
-template<int nt, typename real_t>
-__global__ void __launch_bounds__(nt)
+template<int nt, bool staged, typename real_t>
+__global__ void __launch_bounds__(nt, 1024 / nt)
 sample_k(const real_t* logits, int64_t stride, int vocabulary,
   const float* uniforms, sampling_t settings, int* tokens, int ctas) {
+  extern __shared__ __align__(16) char sample_memory[];
   __shared__ sample_shared_t<nt> shared;
   ptx::cluster_arrive_relaxed();
   int64_t at = (int64_t)blockIdx.x / ctas;
@@ -1035,15 +1173,17 @@ sample_k(const real_t* logits, int64_t stride, int vocabulary,
   int top_k = settings.top_ks ? settings.top_ks[at] : settings.top_k;
   double u = (double)uniforms[at];
 
-  sample_cta_t<nt, real_t> cta(logits + at * stride, vocabulary, shared);
+  typedef sample_cta_t<nt, staged, real_t> cta_t;
+  cta_t cta(logits + at * stride, (typename cta_t::word_t*)sample_memory,
+    vocabulary, shared);
   bool leader = !cta.rank && !cta.tid;
   if(!cta.tid) shared.list_count = 0;
   cta.make_powers();
   cta.log2_scale = 1.4426950408889634 / (double)temperature;
-  cta.inv_temperature = 1.0f / temperature;
+  cta.steps_per_logit = (float)sample_steps / temperature;
   // A part's list holds its greatest top_k and its border's equals.
   bool by_k = temperature > 0 && top_k > 0 && top_k < vocabulary;
-  bool listed = false, peaked = false;
+  bool listed = false, peaked = false, drawable = false;
   double total = -1;
   int count = 0;
   if(by_k && top_k * ctas <= sample_list / 2) {
@@ -1052,6 +1192,8 @@ sample_k(const real_t* logits, int64_t stride, int vocabulary,
   }
   if(!peaked) cta.find_peak();
   cta.peak = key_value(cta.peak_key);
+  // (-infinity has none, whatever the temperature.)
+  cta.weightless = fmaxf(cta.peak - 690.0f * temperature, -FLT_MAX);
   if(0xffffffffu == cta.peak_key || !(cta.peak > -INFINITY)) {
     if(leader) tokens[at] = -1;
   } else if(!(temperature > 0)) {
@@ -1059,15 +1201,17 @@ sample_k(const real_t* logits, int64_t stride, int vocabulary,
     if(leader) tokens[at] = first;
   } else {
     if(by_k && !listed) {
-      listed = cta.template find_border<true>((double)top_k, total, count);
+      listed = cta.template find_border<true>((double)top_k, min_p, total,
+        count, drawable);
       // The weight that top-p refers to is that of the first top_k.
       total = -1;
     }
     bool first_k = listed;
     if(!listed && top_p < 1)
-      listed = cta.template find_border<false>((double)top_p, total, count);
+      listed = cta.template find_border<false>((double)top_p, min_p, total,
+        count, drawable);
     if(!listed)
-      cta.draw(min_p, u, tokens + at);
+      cta.draw(min_p, u, drawable, tokens + at);
     else if(!cta.rank) {
       cta.sort_list(count);
       int token = cta.finish_list(first_k ? min(count, top_k) : count, total,
@@ -1084,10 +1228,22 @@ void sample_enqueue(const real_t* logits, int64_t stride, int count,
   int vocabulary, const float* uniforms, const sampling_t& settings,
   int* tokens, cudaStream_t stream) {
   if(!count) return;
-  enum { nt = 512 };
+  // CTAs to a row: at most 65,536 tokens to a CTA, so that no row takes much
+  // longer than the others (256 mixed rows of 100,003: 224 us with one CTA to a
+  // row, 142 us with two, 151 us with four), and a CTA for each SM where there
+  // are few rows (64 rows of 131,072: 80 us with four, 102 us with eight, whose
+  // clusters need two rounds). Parts up to 72 KB stay in shared memory, which
+  // leaves room for two CTAs on an SM.
+  enum { nt = 512, most_stage = 72 << 10, sms = 148 };
+  auto stage_bytes = [&](int n) {
+    int64_t step = 32 * (16 / (int)sizeof(real_t));
+    return div_up(div_up((int64_t)vocabulary + 8, (int64_t)n * (nt / 32)), step) *
+      step * (nt / 32) * (int64_t)sizeof(real_t);
+  };
   int ctas = 1;
-  while(ctas < sample_max_cluster && (int64_t)count * ctas < 296 &&
-    vocabulary / ctas > 2 * nt) ctas *= 2;
+  while(ctas < sample_max_cluster && vocabulary / ctas > 2 * nt &&
+    ((int64_t)count * ctas < sms || vocabulary / ctas > (1 << 16))) ctas *= 2;
+  bool staged = stage_bytes(ctas) <= most_stage;
   cudaLaunchConfig_t config = { };
   config.gridDim = dim3((unsigned)((int64_t)count * ctas));
   config.blockDim = dim3(nt);
@@ -1098,8 +1254,17 @@ void sample_enqueue(const real_t* logits, int64_t stride, int count,
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  throw_on_error(cudaLaunchKernelEx(&config, sample_k<nt, real_t>, logits,
-    stride, vocabulary, uniforms, settings, tokens, ctas));
+  auto launch = [&](auto kernel) {
+    throw_on_error(cudaLaunchKernelEx(&config, kernel, logits, stride,
+      vocabulary, uniforms, settings, tokens, ctas));
+  };
+  if(staged) {
+    auto kernel = sample_k<nt, true, real_t>;
+    set_dynamic_smem<real_t>(kernel, most_stage);
+    config.dynamicSmemBytes = (size_t)stage_bytes(ctas);
+    launch(kernel);
+  } else
+    launch(sample_k<nt, false, real_t>);
 }
 
 } // namespace detail

@@ -566,6 +566,34 @@ def test_sample_strides(mgpu, dtype, extra, offset):
     check_sample(mgpu, x, 2, top_k=100, top_p=0.9)
 
 
+@pytest.mark.parametrize("settings", [
+    dict(temperature=3e38), dict(temperature=3e38, top_p=0.5),
+    dict(temperature=1e-38), dict(temperature=1e-45, top_p=0.9),
+    dict(temperature=1e30, top_k=3, min_p=0.5)])
+def test_sample_far_temperatures(mgpu, settings):
+    x = sharp(gen(27), 9, 3000, torch.float32)
+    x[:, ::3] = -float("inf")
+    check_sample(mgpu, x, 4, **settings)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("count,vocab", [(1, 300000), (3, 700001), (200, 9000),
+                                         (40, 70001)])
+def test_sample_parts_in_shared_memory_and_not(mgpu, dtype, count, vocab):
+    """Rows of one CTA to eight, parts that stay in shared memory and others."""
+    x = sharp(gen(28), count, vocab, dtype)
+    for i, settings in enumerate([dict(top_p=0.9, min_p=0.001),
+                                  dict(top_k=20), dict(top_k=3000, top_p=0.7)]):
+        check_sample(mgpu, x, i, **settings)
+
+
+def test_sample_nearly_all_of_the_weight(mgpu):
+    """Borders far down, among tokens of next to no weight."""
+    x = randn(gen(29), 12, 20000) * 6
+    for p in (0.99999, 1 - 2.0 ** -24, 1e-7):
+        check_sample(mgpu, x, 6, top_p=p)
+
+
 def test_sample_many_rows(mgpu):
     x = sharp(gen(26), 3000, 257, torch.float16)
     check_sample(mgpu, x, 9, top_p=0.8)
