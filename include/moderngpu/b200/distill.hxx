@@ -490,6 +490,9 @@ distill_stream_k(const real_t* logits, int64_t stride, int count,
           word[i].v[j] = from_f32<real_t>(-INFINITY);
       }
     }
+    // The next copy writes through another proxy than these loads read: without
+    // the fence it overtakes some of them.
+    ptx::fence_proxy_async();
     __syncwarp();
     if(!lane) ptx::mbar_arrive(&shared.empty[stage]);
     next_stage();

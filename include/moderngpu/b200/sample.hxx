@@ -1186,7 +1186,7 @@ sample_k(const real_t* logits, int64_t stride, int vocabulary,
   bool listed = false, peaked = false, drawable = false;
   double total = -1;
   int count = 0;
-  if(by_k && top_k * ctas <= sample_list / 2) {
+  if(by_k && top_k <= sample_list / 2 / ctas) {
     listed = cta.list_greatest(top_k, count);
     peaked = true;
   }

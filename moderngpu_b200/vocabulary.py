@@ -11,8 +11,8 @@ import ctypes
 
 import torch
 
-from .binding import (_DTYPES, _check, _on, _require_cuda, _stream, _workspace,
-                      load_library)
+from .binding import (_DTYPES, _check, _on, _require_cuda, _scratch, _stream,
+                      _workspace, load_library)
 
 F16, BF16 = 4, 5
 _REALS = {torch.float32: _DTYPES[torch.float32], torch.float16: F16,
@@ -122,6 +122,11 @@ def _call_workspace(device, nbytes):
     with _on(device):
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if _raw_stream is not None and device.index is not None:
+        # _workspace's buffer, by the same key.
+        buf = _scratch.get((device.index, _raw_stream(device.index)))
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
     return _workspace(device, nbytes)
 
 

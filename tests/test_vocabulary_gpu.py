@@ -2,6 +2,8 @@
 their definitions in 64 bits (vocabulary_reference.py, which also derives the
 tolerances). Sampled tokens have to be equal."""
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -359,6 +361,23 @@ def test_distill_numbers_of_rows(mgpu, grad_rows, vocab):
     # 32-bit sums of `vocab` weights, and of 20 products of order 30.
     assert torch.allclose(loss.double(), plain, rtol=1e-4, atol=1e-4)
     assert grad.float().sum(1).abs().max() <= 2.0 ** -8 * 2.01
+
+
+@pytest.mark.parametrize("count,vocab,dtype", [
+    (600, 131072, torch.bfloat16), (509, 50021, torch.float32),
+    (2048, 32768, torch.float16)])
+def test_distill_is_the_same_every_time(mgpu, count, vocab, dtype):
+    """Bit for bit: a buffer that is filled again before it has been read would
+    show."""
+    g = gen(20)
+    x = (randn(g, count, vocab) * 3).to(dtype)
+    at, teacher = teacher_of(g, count, vocab, 64)
+    loss, grad = mgpu.distill_loss_gradient(x, at, teacher)
+    for _ in range(25):
+        again = mgpu.distill_loss_gradient(x, at, teacher)
+        assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
+    same = mgpu.distill_loss_gradient(x, at, teacher, out=x)
+    assert torch.equal(same[1], grad) and torch.equal(same[0], loss)
 
 
 def test_distill_rows_without_a_distribution(mgpu):
@@ -764,3 +783,15 @@ def test_refusals(mgpu):
     if torch.cuda.device_count() > 1:
         with pytest.raises(ValueError):
             mgpu.sample_tokens(x, u.to("cuda:1"))
+
+
+def test_cpp_entry_points():
+    """tests/cpp/test_vocabulary.cu: the templates on a context."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp",
+                       "build", "test_vocabulary")
+    if not os.path.exists(exe):
+        pytest.fail("not built: run "
+                    "python -c 'import __graft_entry__ as g; g.build()'")
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert "ALL PASSED" in run.stdout and not run.returncode, (
+        run.stdout + run.stderr)
