@@ -177,7 +177,12 @@ distill_apart_k(const real_t* logits, int64_t stride, int vocabulary,
 // by bulk copies, without a pause between rows: each row (or a CTA's part of it)
 // passes once for its peak and mass and, with want_grad, at once again for the
 // gradient, this time from the L2 (a row for each SM takes 40 MB of it at 2^17
-// logits of 16 bits). HBM sees one read, and one write, of the logits.
+// logits of 16 bits). HBM sees one read, and one write, of the logits, which
+// bounds it: 4,096 x 131,072 bf16 with gradient 430 us, 5.0 TB/s; the loss alone
+// 205 us, 5.2 TB/s. Without the exponentials the former takes 426 us, without the
+// stores 382 us. Clusters that held a row in registers between the passes paid a
+// barrier of eight CTAs for every 256 KB: 570 to 830 us. About 11 us of a call
+// are the first rows' way in and the last ones' out.
 //
 // nt threads take the words; a warp of its own starts the copies, and another one
 // is a row ahead with the teacher: it reduces the entries to what the CTA needs

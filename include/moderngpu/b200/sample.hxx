@@ -77,6 +77,10 @@ MGPU_DEVICE __forceinline__ float key_value(uint32_t key) {
 // What a warp finds it tells all CTAs at once, and every warp adds up what all
 // warps told: one barrier of the cluster (1,300 cycles) to an exchange, and none
 // of the CTA.
+//
+// Not bound by bytes: one row of 131,072 takes 16 us by the latency of some eight
+// exchanges and of the list; 64 rows of them under top-p alone 80 us by the
+// instructions of passes 2 and 3, of which a fourth are operations of 64 bits.
 
 enum { sample_bins = 2048, sample_steps = 64, sample_list = 1024,
   sample_max_cluster = 8, sample_powers = 64, sample_groups = 64 };

@@ -309,7 +309,8 @@ int mgpu_b200_embedding_gradient(int dtype, const void* grad_device,
  * An entry whose token is outside of [0, vocabulary) is unused; a token may
  * occur in several entries. A row without an entry above -infinity, a row
  * whose logits are all -infinity and a row of weight 0 have loss 0 and
- * gradient 0 (the logits of the first and the last are not read). `weights`
+ * gradient 0, whatever else they hold. A copy that does not arrive within two
+ * seconds ends the wait for it: the rows' losses and gradients are NaN. `weights`
  * may be NULL: 1 for every row. grad may be logits itself (same stride), and
  * must not overlap it otherwise. T > 0.
  */

@@ -236,7 +236,7 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
     (loss, out), out[i] = row_weights[i] * d loss[i] / d logits[i], of the
     logits' dtype. row_weights (float32; 1 where not given) is what a training
     step multiplies each row's loss by, such as 1 / count; a row of weight 0 is
-    masked: loss 0, gradient 0, and its logits are not read. `out` may be
+    masked: loss 0 and gradient 0, whatever its logits are. `out` may be
     `logits` itself, which then holds the gradient.
     """
     lib = load_library()
