@@ -228,8 +228,11 @@ token_scatter_k(source_t source, int count, int shift, int tiles,
     int64_t i = first + j * 32 + lane;
     if(i < count) {
       int to = seen[warp][(keys[j] >> shift) & (token_digits - 1)] + places[j];
-      keys_out[to] = keys[j];
-      positions_out[to] = source.position((int)i);
+      // Within the array also where the scan has given up.
+      if((unsigned)to < (unsigned)count) {
+        keys_out[to] = keys[j];
+        positions_out[to] = source.position((int)i);
+      }
     }
   }
 }
@@ -552,7 +555,9 @@ embedding_sum_k(const real_t* grad, int64_t stride, int width, int slab,
   int entries = end - begin;
   for(int e = tid; e < entries; e += nt) {
     tile_keys[e] = keys[begin + e];
-    tile_positions[e] = positions[begin + e];
+    // In range also where a scan of the sort has given up (status word).
+    tile_positions[e] = (int)min((uint32_t)positions[begin + e],
+      (uint32_t)count - 1);
   }
   uint32_t row = keys[begin];
   if(row >= (uint32_t)rows) return;
@@ -601,7 +606,7 @@ embedding_sum_k(const real_t* grad, int64_t stride, int width, int slab,
           int place = (e + i) % depth * nt;
           ptx::cp_async<(int)sizeof(word_t)>(ring + place, from_row(e + i));
           if constexpr (staged_out)
-            if(begins(e + i)) {
+            if(begins(e + i) && tile_keys[e + i] < (uint32_t)rows) {
               const out_part_t* from = out_row(tile_keys[e + i]);
               enum { size = sizeof(from->words[0]) };
               #pragma unroll
@@ -629,6 +634,7 @@ embedding_sum_k(const real_t* grad, int64_t stride, int width, int slab,
     atomicMin(&told_to, tile + tid);
   out_part_t old;
   auto store = [&](uint32_t r) {
+    if(r >= (uint32_t)rows) return;
     if constexpr (accumulate && !staged_out) old = *out_row(r);
     store_row_part<accumulate>((out_t*)out_row(r), sum, scale, old);
   };
@@ -741,9 +747,11 @@ embedding_sum_k(const real_t* grad, int64_t stride, int width, int slab,
   }
 }
 
-// Sizes and scratch of a call: the sorted pairs (two sets and the digit counts
-// with their scan where one cluster does not take them), the partial sums and
-// their counters.
+// Sizes and scratch of a call: a header with the status word that every
+// workspace has (the scan's, where one runs; else 0), the counters behind it,
+// the sorted pairs (two sets and the digit counts where one cluster does not take
+// them) and the partial sums.
+enum { embedding_header = 32 };              // words
 struct embedding_plan_t {
   int tile_size, tiles, vt, ctas, sort_tiles;
   int64_t sums;
@@ -774,6 +782,11 @@ struct embedding_plan_t {
       at += (n + 127) / 128 * 128;
       return here;
     };
+    int cells = sort_tiles * token_digits;
+    scan = take(ctas ? 4 * embedding_header : scan_workspace_bytes<
+      typename scan_default_tuning<int>::type, int>(cells));
+    // A slab has about embedding_nt columns at least.
+    counters = take(4 * (size_t)sums * div_up(width, (int)embedding_nt));
     for(int i = 0; i < (ctas ? 1 : 2); ++i) {
       keys[i] = take(4 * (size_t)count);
       positions[i] = take(4 * (size_t)count);
@@ -782,13 +795,8 @@ struct embedding_plan_t {
       keys[1] = keys[0];
       positions[1] = positions[0];
     }
-    int cells = sort_tiles * token_digits;
     counts = take(4 * (size_t)cells);
-    scan = take(ctas ? 0 : scan_workspace_bytes<
-      typename scan_default_tuning<int>::type, int>(cells));
     parts = take(4 * (size_t)sums * width);
-    // A slab has about embedding_nt columns at least.
-    counters = take(4 * (size_t)sums * div_up(width, (int)embedding_nt));
     bytes = at;
   }
 };
@@ -860,13 +868,15 @@ void embedding_gradient_enqueue(const real_t* grad, int64_t stride, int width,
   token_keys_t<token_t> source { tokens, rows };
 
   int into = 0;
+  if(!count)
+    embedding_clear_k<256><<<1, 256, 0, stream>>>((int*)base, embedding_header);
   if(count && plan.ctas) {
     if(8 == plan.vt)
       token_cluster_sort<8>(plan, source, count, keys[0], positions[0],
-        counters, num_counters, stream);
+        (int*)base, embedding_header + num_counters, stream);
     else
       token_cluster_sort<32>(plan, source, count, keys[0], positions[0],
-        counters, num_counters, stream);
+        (int*)base, embedding_header + num_counters, stream);
   } else if(count) {
     typedef scan_route_t<empty_t, int, int*, int*> route_t;
     int* counts = (int*)(base + plan.counts);

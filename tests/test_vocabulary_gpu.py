@@ -187,6 +187,25 @@ def test_gradient_of_nothing(mgpu):
     assert mgpu.embedding_gradient(grad, tokens, 0).shape == (0, 8)
 
 
+@pytest.mark.parametrize("count", [0, 1, 5000, 140000])
+def test_gradient_leaves_a_status_in_its_workspace(mgpu, count):
+    """The word that workspace_status reads, here in a workspace full of ones,
+    and in the stream's own between calls that share it."""
+    g = gen(count)
+    tokens = tokens_of(g, count, 3000)
+    grad = randn(g, count, 8)
+    need = mgpu.load_library().mgpu_b200_embedding_gradient_workspace_bytes(
+        count, 3000, 8, 0)
+    workspace = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    want = mgpu.embedding_gradient(grad, tokens, 3000, workspace=workspace)
+    assert mgpu.workspace_status(workspace) == 0
+    assert torch.equal(mgpu.embedding_gradient(grad, tokens, 3000), want)
+    assert mgpu.workspace_status() == 0
+    x = torch.arange(1000, dtype=torch.int32, device="cuda")
+    assert torch.equal(mgpu.scan(x, inclusive=True), torch.cumsum(x, 0).int())
+    assert mgpu.workspace_status() == 0
+
+
 def test_gradient_leaves_out_padding_whatever_it_holds(mgpu):
     grad = randn(gen(5), 200, 64)
     tokens = tokens_of(gen(5), 200, 50)
