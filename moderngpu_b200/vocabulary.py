@@ -53,10 +53,11 @@ def declare(lib):
         c_void_p]
 
 
-# The address of the current stream without the Stream object around it, which
-# costs as much as the launch of a small kernel; the public way where a torch
-# does not have it.
+# The address of the current stream and the number of the current device without
+# the objects around them, which cost as much as the launch of a small kernel; the
+# public ways where a torch does not have these.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _stream_of(device):
@@ -65,9 +66,23 @@ def _stream_of(device):
     return _raw_stream(device.index)
 
 
+def _call(device, entry, *arguments):
+    """entry(*arguments, current stream) with `device` the current one; raises
+    MgpuError."""
+    if _raw_device is not None and device.index == _raw_device():
+        code = entry(*arguments, _stream_of(device))
+    else:
+        with _on(device):
+            code = entry(*arguments, _stream_of(device))
+    if code:
+        _check(code)
+
+
 def _require(t, name, dtypes, device=None):
     """A dense CUDA tensor of one of the dtypes, on the call's device."""
-    _require_cuda(t, name)
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or \
+            not t.is_contiguous():
+        _require_cuda(t, name)
     if t.dtype not in dtypes:
         raise TypeError("%s must have one of the dtypes %s" %
                         (name, ", ".join(str(d) for d in dtypes)))
@@ -119,9 +134,13 @@ def _call_workspace(device, nbytes):
     """The stream's scratch buffer; while a graph is captured, memory of the
     graph's own, so that graphs which are replayed at the same time share
     none."""
-    with _on(device):
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if _raw_device is not None and device.index == _raw_device():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with _on(device):
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     if _raw_stream is not None and device.index is not None:
         # _workspace's buffer, by the same key.
         buf = _scratch.get((device.index, _raw_stream(device.index)))
@@ -138,16 +157,15 @@ def embedding_lookup(table, tokens, scale=1.0, out=None):
     of any shape; out: tokens.shape + (width,), of the table's dtype.
     """
     lib = load_library()
-    dtype, device = table.dtype, table.device
     rows, width, stride = _matrix(table, "table", _REALS)
+    dtype, device = table.dtype, table.device
     _require(tokens, "tokens", _TOKENS, device)
     count = _fits(tokens.numel(), "tokens")
     out = _shaped(out, "out", tokens.shape + (width,), (dtype,), device)
-    with _on(device):
-        _check(lib.mgpu_b200_embedding_lookup(
-            _REALS[dtype], table.data_ptr(), rows, width, stride,
-            _TOKENS[tokens.dtype], tokens.data_ptr(), count, scale,
-            out.data_ptr(), _stream_of(device)))
+    _call(device, lib.mgpu_b200_embedding_lookup,
+          _REALS[dtype], table.data_ptr(), rows, width, stride,
+          _TOKENS[tokens.dtype], tokens.data_ptr(), count, scale,
+          out.data_ptr())
     return out
 
 
@@ -186,12 +204,11 @@ def embedding_gradient(grad, tokens, rows, scale=1.0, out=None,
                 count, rows, width, int(accumulate)))
     else:
         _require(workspace, "workspace", (torch.uint8,), device)
-    with _on(device):
-        _check(lib.mgpu_b200_embedding_gradient(
-            _REALS[grad.dtype], grad.data_ptr(), stride, width,
-            _TOKENS[tokens.dtype], tokens.data_ptr(), count, rows, scale,
-            int(accumulate), _REALS[out.dtype], out.data_ptr(),
-            workspace.data_ptr(), workspace.numel(), _stream_of(device)))
+    _call(device, lib.mgpu_b200_embedding_gradient,
+          _REALS[grad.dtype], grad.data_ptr(), stride, width,
+          _TOKENS[tokens.dtype], tokens.data_ptr(), count, rows, scale,
+          int(accumulate), _REALS[out.dtype], out.data_ptr(),
+          workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -216,16 +233,15 @@ def distill_loss(logits, teacher_tokens, teacher_logits, temperature=1.0,
     teacher_logits: of the same shape, any of the three dtypes.
     """
     lib = load_library()
-    device = logits.device
     count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    device = logits.device
     entries = _teacher(count, device, teacher_tokens, teacher_logits)
     out = _shaped(out, "out", (count,), (torch.float32,), device)
-    with _on(device):
-        _check(lib.mgpu_b200_distill_loss(
-            _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
-            _TOKENS[teacher_tokens.dtype], teacher_tokens.data_ptr(),
-            _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
-            temperature, out.data_ptr(), _stream_of(device)))
+    _call(device, lib.mgpu_b200_distill_loss,
+          _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
+          _TOKENS[teacher_tokens.dtype], teacher_tokens.data_ptr(),
+          _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
+          temperature, out.data_ptr())
     return out
 
 
@@ -240,8 +256,8 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
     `logits` itself, which then holds the gradient.
     """
     lib = load_library()
-    device = logits.device
     count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    device = logits.device
     entries = _teacher(count, device, teacher_tokens, teacher_logits)
     loss = _shaped(loss, "loss", (count,), (torch.float32,), device)
     if row_weights is not None:
@@ -254,14 +270,13 @@ def distill_loss_gradient(logits, teacher_tokens, teacher_logits,
     _, _, out_stride = _matrix(out, "out", (logits.dtype,), device)
     if out.shape != logits.shape:
         raise ValueError("out must have the logits' shape")
-    with _on(device):
-        _check(lib.mgpu_b200_distill_loss_gradient(
-            _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
-            _TOKENS[teacher_tokens.dtype], teacher_tokens.data_ptr(),
-            _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
-            temperature, None if row_weights is None else
-            row_weights.data_ptr(), loss.data_ptr(), out.data_ptr(),
-            out_stride, _stream_of(device)))
+    _call(device, lib.mgpu_b200_distill_loss_gradient,
+          _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
+          _TOKENS[teacher_tokens.dtype], teacher_tokens.data_ptr(),
+          _REALS[teacher_logits.dtype], teacher_logits.data_ptr(), entries,
+          temperature, None if row_weights is None else
+          row_weights.data_ptr(), loss.data_ptr(), out.data_ptr(),
+          out_stride)
     return loss, out
 
 
@@ -288,20 +303,20 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0,
     without a logit above -infinity gives -1.
     """
     lib = load_library()
-    device = logits.device
     count, vocabulary, stride = _matrix(logits, "logits", _REALS)
+    device = logits.device
     _require(uniform, "uniform", (torch.float32,), device)
     if tuple(uniform.shape) != (count,):
         raise ValueError("uniform must have one number for each row")
     t, t_rows = _setting(temperature, "temperature", torch.float32, count,
                          device)
     k, k_rows = _setting(top_k, "top_k", torch.int32, count, device)
+    k = max(min(k, _MOST), 0)
     p, p_rows = _setting(top_p, "top_p", torch.float32, count, device)
     m, m_rows = _setting(min_p, "min_p", torch.float32, count, device)
     out = _shaped(out, "out", (count,), (torch.int32,), device)
-    with _on(device):
-        _check(lib.mgpu_b200_sample_tokens(
-            _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
-            uniform.data_ptr(), t, t_rows, k, k_rows, p, p_rows, m, m_rows,
-            out.data_ptr(), _stream_of(device)))
+    _call(device, lib.mgpu_b200_sample_tokens,
+          _REALS[logits.dtype], logits.data_ptr(), stride, count, vocabulary,
+          uniform.data_ptr(), t, t_rows, k, k_rows, p, p_rows, m, m_rows,
+          out.data_ptr())
     return out

@@ -799,6 +799,15 @@ def test_refusals(mgpu):
         mgpu.sample_tokens(x, u, top_p=u[:2])
     with pytest.raises(mgpu.MgpuError):
         mgpu.sample_tokens(x, u, temperature=-1.0)
+    for call in (lambda: mgpu.embedding_lookup([1], i),
+                 lambda: mgpu.embedding_gradient(None, i, 4),
+                 lambda: mgpu.distill_loss(3, at, x),
+                 lambda: mgpu.sample_tokens("x", u)):
+        with pytest.raises(TypeError):
+            call()
+    # More tokens than there are: all of them.
+    assert torch.equal(mgpu.sample_tokens(x, u, top_k=2**40),
+                       mgpu.sample_tokens(x, u))
     if torch.cuda.device_count() > 1:
         with pytest.raises(ValueError):
             mgpu.sample_tokens(x, u.to("cuda:1"))
