@@ -189,10 +189,11 @@ distill_apart_k(const real_t* logits, int64_t stride, int vocabulary,
 // of them, the list of tokens in its part with their probabilities and the
 // student's logits, and of p and p (s - the greatest of these logits) the sums,
 // which is all that the loss needs: log q_j = (s_j - peak) / T - log mass.
-// A row of many words has a CTA of 512 threads, one to an SM; rows of less are
-// worked on by four CTAs of 128, whose barriers hide behind one another.
+// Long rows are worked on by two CTAs of 256 threads on each SM, shorter ones by
+// four of 128: their barriers hide behind one another.
 enum { distill_words = 4,          // a thread's words in a landing buffer
-  distill_nt_large = 512, distill_nt_small = 128, distill_small_per_sm = 4 };
+  distill_nt_large = 256, distill_large_per_sm = 2, distill_nt_small = 128,
+  distill_small_per_sm = 4 };
 
 struct distill_list_t {
   int listed, taught;
@@ -282,8 +283,8 @@ MGPU_DEVICE __forceinline__ float words_peak(
 }
 
 template<int nt, int pack, bool want_grad, typename real_t>
-__global__ void __launch_bounds__(nt + 64, nt == distill_nt_large ? 1 :
-  distill_small_per_sm)
+__global__ void __launch_bounds__(nt + 64, nt == distill_nt_large ?
+  distill_large_per_sm : distill_small_per_sm)
 distill_stream_k(const real_t* logits, int64_t stride, int count,
   int vocabulary, int log_ctas, int stages, distill_teacher_t teacher,
   float temperature, const float* weights, float* losses, real_t* grad,
@@ -693,7 +694,8 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
   }
   auto launch = [&](auto threads) {
     enum { nt = decltype(threads)::value,
-      per_sm = nt == distill_nt_large ? 1 : distill_small_per_sm,
+      per_sm = nt == distill_nt_large ? distill_large_per_sm :
+        distill_small_per_sm,
       stage_bytes = nt * distill_words * 16 };
     auto kernel = distill_stream_k<nt, 16 / (int)size, want_grad, real_t>;
     // What an SM has, less the shared variables of fixed size.
@@ -706,7 +708,8 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
     config.blockDim = dim3(nt + 64);
     config.dynamicSmemBytes = (size_t)stages * stage_bytes + lists;
     // CTAs to a row: rounds of rows times what each takes, a round's barriers
-    // being worth about 32 KB.
+    // being worth about 32 KB. The second pass finds the row in the L2 only
+    // where the rows under way take no more than half of it.
     int ctas = 1, clusters = 1;
     int64_t least = 0;
     for(int n = 1; n <= distill_max_cluster; n *= 2) {
@@ -716,7 +719,9 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
         bool, want_grad>, real_t>(kernel, config, n, stages);
       int64_t cost = div_up((int64_t)count, (int64_t)most) *
         (row_bytes / n + (32 << 10));
-      if(!least || cost < least) {
+      bool crowded = want_grad && distill_max_cluster != n &&
+        min(count, most) * row_bytes > (64 << 20);
+      if(!crowded && (!least || cost < least)) {
         least = cost;
         ctas = n;
         clusters = most;
@@ -729,10 +734,10 @@ void distill_enqueue(const real_t* logits, int64_t stride, int count,
       vocabulary, log_ctas, stages, source, temperature, weights, losses, grad,
       grad_stride, timeout_ns));
   };
-  // Measured with 2,048 rows of 64 KB (loss): 30.5 us in small CTAs, 57.8 us in
-  // large ones; with gradient, 509 rows of 200 KB: 61 us small, 46 us large, and
-  // 4,096 rows of 256 KB: 565 us small (150 MB of rows under way push one another
-  // out of the L2), 426 us large.
+  // Measured with 2,048 rows of 64 KB (loss): 30.5 us in small CTAs, 36 us in
+  // large ones; with gradient, 509 rows of 200 KB: 61 us small, 43 us large, and
+  // 4,096 rows of 256 KB: 565 us small, 425 us large, 525 us with 75 MB of rows
+  // under way. One CTA of 512 threads to an SM took 47 us and 432 us.
   if(row_bytes > (96 << 10))
     launch(std::integral_constant<int, distill_nt_large>());
   else
