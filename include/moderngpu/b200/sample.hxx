@@ -826,16 +826,19 @@ struct sample_cta_t {
       count = (int)__reduce_max_sync(0xffffffffu, fit);
     }
     double upto_mine[4] = { 0, 0, 0, 0 };
+    int index[4];
+    #pragma unroll
+    for(int i = 0; i < 4; ++i)
+      index[i] = lane * 4 + i < count ? list_index(lane * 4 + i) : -1;
     sum = 0;
+    #pragma unroll 4
     for(int q = 0; q < count; ++q) {
       double w = shared.list_weights[q];
       int at = list_index(q);
       sum += w;
       #pragma unroll
-      for(int i = 0; i < 4; ++i) {
-        int e = lane * 4 + i;
-        if(e < count && at <= list_index(e)) upto_mine[i] += w;
-      }
+      for(int i = 0; i < 4; ++i)
+        upto_mine[i] += at <= index[i] ? w : 0.0;
     }
     double target = u * sum;
     uint32_t hit = 0xffffffffu, any = 0;
@@ -843,7 +846,7 @@ struct sample_cta_t {
     for(int i = 0; i < 4; ++i) {
       int e = lane * 4 + i;
       if(e < count && own[i] > 0) {
-        uint32_t at = (uint32_t)list_index(e);
+        uint32_t at = (uint32_t)index[i];
         any = max(any, at);
         if(upto_mine[i] > target) hit = min(hit, at);
       }

@@ -578,6 +578,26 @@ def test_sample_masks(mgpu, dtype, settings):
     assert got[1] == 4999 and got[2] == -1 and got[3] == -1
 
 
+@pytest.mark.parametrize("dtype", REALS)
+def test_sample_top_k_of_unlike_parts(mgpu, dtype):
+    """The greatest tokens in one part of the row, spread over all, equal, far
+    apart, large against their distances, and infinite."""
+    x = randn(gen(30), 10, 40000, dtype=dtype)
+    x[0, 39000:39100] = 30.0
+    x[1, ::400] = 12.0
+    x[2] = 0.0
+    x[3] = torch.arange(40000, device="cuda") % 977 / 8
+    x[4] = 3e4 + torch.arange(40000, device="cuda") % 50
+    x[5, 7::5000] = float("inf")
+    x[6, :20000] = -float("inf")
+    x[7] = -float("inf")
+    x[7, 5::9000] = 1.0
+    x[8, 100:200] = float("inf")
+    for k in (1, 3, 50, 64, 200):
+        for t in (1.0, 0.01, 100.0):
+            check_sample(mgpu, x, k, top_k=k, temperature=t)
+
+
 def test_sample_top_k_beyond_the_tokens_left(mgpu):
     x = torch.full((4, 3000), -float("inf"), device="cuda")
     x[:, 2000:2005] = torch.randn(4, 5, device="cuda", generator=gen(23))
