@@ -252,6 +252,16 @@ def test_gradient_of_many_positions(mgpu):
                    30011, out_dtype=torch.float32)
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("count,rows", [(32769, 900), (131072, 511),
+                                        (131073, 70000), (300001, 300000)])
+def test_gradient_of_each_form_of_the_sort(mgpu, count, rows, accumulate):
+    """Around the numbers of positions that one cluster takes."""
+    g = gen(count)
+    check_gradient(mgpu, randn(g, count, 12), tokens_of(g, count, rows), rows,
+                   accumulate=accumulate)
+
+
 def test_gradient_against_differences_of_the_lookup(mgpu):
     """The lookup is linear: <lookup(d), grad> = <d, gradient(grad)>."""
     g = gen(10)
